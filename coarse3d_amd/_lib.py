@@ -59,7 +59,32 @@ class PackEntry(C.Structure):
                 ("Kpad", C.c_int32), ("reserved", C.c_int32)]
 
 
+class OptTensor(C.Structure):
+    _fields_ = [("ptr", C.c_void_p * 7), ("n", C.c_int64)]
+
+
+class AdamWDesc(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+                ("grad_scale", C.c_void_p), ("step_dev", C.c_void_p), ("lr_dev", C.c_void_p), ("step", C.c_int64),
+                ("param_type", C.c_int32), ("grad_type", C.c_int32), ("state_bits", C.c_int32), ("has_master", C.c_int32),
+                ("seed", C.c_uint32), ("reserved", C.c_int32)]
+
+
 _lib = None
+_tlist = None
+
+
+def tensor_list():
+    """The native module that turns lists of tensors into the records of the many-tensor entry points (csrc/tensor_list.cpp)."""
+    global _tlist
+    if _tlist is None:
+        try:
+            from . import _tensor_list
+        except ImportError as e:
+            raise RuntimeError("coarse3d_amd/_tensor_list.so is missing or does not load: the extension has not been built (run "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`). There is no fallback.") from e
+        _tlist = _tensor_list
+    return _tlist
 
 
 def lib():

@@ -715,6 +715,238 @@ def sums_to_f32(sums, col, out, accumulate=False):
     return out
 
 
+def _call_on(index, name, *args):
+    """``_call`` on the device that the tensors live on, on that device's current stream."""
+    if index == _cur_dev():
+        _call(name, *args, _stream())
+    else:
+        with torch.cuda.device(index):
+            _call(name, *args, _stream())
+
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+# ---------------------------------------------------------------------------- GroupNorm with an activation
+_ACTS = {"none": 0, "lrelu": 1, "silu": 2}
+
+
+def _pixel_rows(t, what):
+    """(samples, pixels, channels, elements from sample to sample, from pixel to pixel) of a channels-last tensor [N, ..., C]."""
+    if t.dim() < 2:
+        raise ValueError(f"{what} is [N, ..., C], got {tuple(t.shape)}")
+    n, c = t.shape[0], t.shape[-1]
+    if t.numel() == 0:
+        return n, (0 if c and n else 1), c, 0, c
+    if t.is_contiguous():
+        hw = t.numel() // (n * c)
+        return n, hw, c, hw * c, c
+    st, hw, ps = t.stride(), 1, None
+    ok = c == 1 or st[-1] == 1
+    for d in range(t.dim() - 2, 0, -1):
+        if t.shape[d] > 1:
+            if ps is None:
+                ps = st[d]
+            ok = ok and st[d] == ps * hw
+            hw *= t.shape[d]
+    ps = c if ps is None else ps
+    ns = st[0] if n > 1 else hw * ps
+    if not ok or ps < c or (n > 1 and ns < (hw - 1) * ps + c):
+        raise ValueError(f"{what}: the channels of a pixel have to lie side by side and the pixels one stride apart; got shape "
+                         f"{tuple(t.shape)}, strides {st} (call .contiguous())")
+    return n, hw, c, ns, ps
+
+
+def _affine_vectors(gamma, beta, c, device):
+    for t, name in ((gamma, "gamma"), (beta, "beta")):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (c,) or not t.is_contiguous() or t.device != device):
+            raise ValueError(f"group_norm: {name} is a contiguous fp32 tensor of {c} values on {device}")
+
+
+def _gn_check(x, act, slope, what):
+    if x.dtype not in _TYPES:
+        raise ValueError(f"{what}: fp32, bf16 or fp16, got {x.dtype}")
+    if act not in _ACTS:
+        raise ValueError(f"{what}: act is one of {sorted(_ACTS)}, got {act!r}")
+    if not 0.0 <= slope <= 1.0:
+        raise ValueError(f"{what}: slope is in [0, 1], got {slope}")
+
+
+def _on_gpu(t, what):
+    if not t.is_cuda:
+        raise ValueError(f"{what}: the tensors are on {t.device}, not on a GPU")
+
+
+def group_norm(x, groups, gamma=None, beta=None, eps=1e-5, act="lrelu", slope=0.01):
+    """act(GroupNorm(x)) over a channels-last image: x [N, ..., C] (fp32, bf16 or fp16; a channel slice or a cropped batch of a
+    larger tensor is fine), statistics over the pixels and the C / groups channels of each (sample, group), gamma / beta [C] fp32
+    or None.  act: "none", "lrelu" (``slope``; 0 = ReLU) or "silu".  Returns (y, mean, rstd): y dense and of x's type, mean / rstd
+    [N, groups] fp32 for ``group_norm_bwd``.  Sums are fp32 or wider, y is rounded once.  A sample that holds a value which is not
+    finite gives NaN in that value's group and nowhere else."""
+    _gn_check(x, act, slope, "group_norm")
+    n, hw, c, ns, ps = _pixel_rows(x, "group_norm: x")
+    if groups < 1 or c < 1 or c % groups:
+        raise ValueError(f"group_norm: {c} channels do not divide into {groups} groups")
+    if not eps >= 0.0:
+        raise ValueError(f"group_norm: eps is not negative, got {eps}")
+    _affine_vectors(gamma, beta, c, x.device)
+    _on_gpu(x, "group_norm")
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    if n == 0 or hw == 0:
+        return y, torch.zeros(n, groups, device=x.device), torch.zeros(n, groups, device=x.device)
+    ty = _TYPES[x.dtype]
+    stats = torch.empty(2, n, groups, device=x.device, dtype=torch.float32)
+    mean, rstd = stats[0], stats[1]
+    ws = torch.empty(L.lib().c3d_group_norm_ws_floats(n, hw, c, groups, ty), device=x.device, dtype=torch.float32)
+    _call_on(x.get_device(), "c3d_group_norm", _dp(x), ns, ps, n, hw, c, groups, ty, _dp(gamma), _dp(beta), eps, _ACTS[act], slope, _dp(y), _dp(mean),
+             _dp(rstd), _dp(ws))
+    return y, mean, rstd
+
+
+def group_norm_bwd(dy, x, mean, rstd, gamma=None, beta=None, act="lrelu", slope=0.01):
+    """Gradients of ``group_norm``: (dx, dgamma, dbeta), dx dense and of x's type, dgamma / dbeta [C] fp32 (None where the
+    parameter is None).  Deterministic: partial sums are folded in a fixed order."""
+    _gn_check(x, act, slope, "group_norm_bwd")
+    n, hw, c, ns, ps = _pixel_rows(x, "group_norm_bwd: x")
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError(f"group_norm_bwd: dy is {tuple(dy.shape)} {dy.dtype} on {dy.device}, x is {tuple(x.shape)} {x.dtype} on {x.device}")
+    _, _, _, dns, dps = _pixel_rows(dy, "group_norm_bwd: dy")
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t.dim() != 2 or t.shape[0] != n or t.shape != mean.shape or t.dtype != torch.float32 or not t.is_contiguous() or t.device != x.device:
+            raise ValueError(f"group_norm_bwd: {name} is the fp32 [N, groups] tensor that group_norm returned")
+    groups = mean.shape[1]
+    if groups < 1 or c < 1 or c % groups:
+        raise ValueError(f"group_norm_bwd: {c} channels do not divide into {groups} groups")
+    _affine_vectors(gamma, beta, c, x.device)
+    _on_gpu(x, "group_norm_bwd")
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    if n == 0 or hw == 0:
+        z = torch.zeros(2, c, device=x.device)
+        return dx, z[0] if gamma is not None else None, z[1] if beta is not None else None
+    ty = _TYPES[x.dtype]
+    dgamma = torch.empty(c, device=x.device, dtype=torch.float32) if gamma is not None else None
+    dbeta = torch.empty(c, device=x.device, dtype=torch.float32) if beta is not None else None
+    ws = torch.empty(L.lib().c3d_group_norm_ws_floats(n, hw, c, groups, ty), device=x.device, dtype=torch.float32)
+    _call_on(x.get_device(), "c3d_group_norm_bwd", _dp(dy), dns, dps, _dp(x), ns, ps, n, hw, c, groups, ty, _dp(mean), _dp(rstd), _dp(gamma), _dp(beta),
+             _ACTS[act], slope, _dp(dx), _dp(dgamma), _dp(dbeta), _dp(ws))
+    return dx, dgamma, dbeta
+
+
+# ---------------------------------------------------------------------------- optimiser over many tensors
+ADAMW8_BLOCK = 256       # elements of an 8-bit state that share a scale (C3D_ADAMW8_BLOCK)
+_GRAD_NAMES = ("", "grads", "", "", "", "", "")
+
+
+def _grad_records(grads, kind, what):
+    buf, n, index, types = L.tensor_list().pack(what, (None, grads, None, None, None, None, None), "w" + kind + "wwwww", _GRAD_NAMES)
+    if n == 0:
+        raise ValueError(f"{what}: no tensors")
+    if types[1] not in _TYPES:
+        raise ValueError(f"{what}: gradients are fp32, bf16 or fp16, got {types[1]}")
+    return buf, n, index, _TYPES[types[1]]
+
+
+def _grad_norm(records, max_norm, what):
+    if not max_norm >= 0.0:
+        raise ValueError(f"{what}: max_norm is not negative, got {max_norm}")
+    buf, n, index, ty = records
+    dev = torch.device("cuda", index)
+    part = torch.empty(L.lib().c3d_grad_norm_partials(buf, n), device=dev, dtype=torch.float64)
+    out = torch.empty(2, device=dev, dtype=torch.float32)
+    norm, scale = out[0], out[1]
+    _call_on(index, "c3d_grad_norm", buf, n, ty, max_norm, _dp(part), _dp(norm), _dp(scale))
+    return norm, scale
+
+
+def grad_norm(grads, max_norm=float("inf")):
+    """(norm, scale): the 2-norm over all values of a list of tensors of one type, and min(1, max_norm / (norm + 1e-6)) -- the factor
+    of ``torch.nn.utils.clip_grad_norm_`` -- as 0-dim fp32 device tensors; nothing waits for them.  ``scale`` is what ``adamw_step``
+    takes as ``grad_scale``: clipping then costs no pass of its own.  Squares and sums are 64 bits wide.  A gradient that is not
+    finite gives a norm that is not finite (and a scale of 0 or NaN), as in torch."""
+    return _grad_norm(_grad_records(grads, "r", "grad_norm"), float(max_norm), "grad_norm")
+
+
+def clip_grad_norm_(grads, max_norm):
+    """Scales a list of gradients in place such that their joint 2-norm is at most ``max_norm``; returns the norm they had."""
+    records = _grad_records(grads, "w", "clip_grad_norm_")
+    norm, scale = _grad_norm(records, float(max_norm), "clip_grad_norm_")
+    buf, n, index, ty = records
+    _call_on(index, "c3d_scale_tensors", buf, n, ty, _dp(scale))
+    return norm
+
+
+def _device_scalar(t, index, what):
+    if t.numel() != 1 or t.dtype != torch.float32 or t.get_device() != index:
+        raise ValueError(f"{what} as a tensor is one fp32 value on the parameters' device")
+    return t.data_ptr()
+
+
+def _adamw(what, lists, kinds, names, bits, step, lr, betas, eps, weight_decay, grad_scale, seed):
+    buf, n, index, types = L.tensor_list().pack(what, lists, kinds, names)
+    if n == 0:
+        raise ValueError(f"{what}: no tensors")
+    p, g, m, v, ms, vs, w = types
+    if p not in _TYPES or g not in (p, torch.float32):
+        raise ValueError(f"{what}: parameters are fp32, bf16 or fp16 and gradients of the same type or fp32, got {p} and {g}")
+    want = torch.float32 if bits == 32 else torch.float8_e4m3fn
+    if m != want or v != want:
+        raise ValueError(f"{what}: the states are {want}, got {m} and {v}")
+    if bits == 8 and (ms != torch.float32 or vs != torch.float32):
+        raise ValueError(f"{what}: the states' scales are fp32, got {ms} and {vs}")
+    if w is not None and (w != torch.float32 or p == torch.float32):
+        raise ValueError(f"{what}: master copies are fp32, of 16-bit parameters; got {w} of {p}")
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+        raise ValueError(f"{what}: betas are in [0, 1), got {betas}")
+    if not eps >= 0.0:
+        raise ValueError(f"{what}: eps is not negative, got {eps}")
+    d = L.AdamWDesc()
+    if isinstance(lr, torch.Tensor):
+        d.lr_dev = _device_scalar(lr, index, f"{what}: lr")
+    else:
+        d.lr = lr
+    if isinstance(step, torch.Tensor):
+        d.step_dev = _device_scalar(step, index, f"{what}: step")
+    elif step < 1:
+        raise ValueError(f"{what}: step counts from 1, got {step}")
+    else:
+        d.step = step
+    if grad_scale is not None:
+        d.grad_scale = _device_scalar(grad_scale, index, f"{what}: grad_scale")
+    d.beta1, d.beta2, d.eps, d.weight_decay = betas[0], betas[1], eps, weight_decay
+    d.param_type, d.grad_type, d.state_bits, d.has_master, d.seed = _TYPES[p], _TYPES[g], bits, int(w is not None), seed & 0xFFFFFFFF
+    _call_on(index, "c3d_adamw_step", buf, n, C.byref(d))
+
+
+_ADAMW_NAMES = ("params", "grads", "exp_avgs", "exp_avg_sqs", "", "", "masters")
+_ADAMW8_NAMES = ("params", "grads", "exp_avgs", "exp_avg_roots", "exp_avg_scales", "exp_avg_root_scales", "masters")
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, grad_scale=None,
+               masters=None):
+    """One AdamW step (torch.optim.AdamW's formula) over lists of tensors, in place, in as few launches as the kernel arguments
+    allow (88 tensors each; 72 with masters).
+
+    params fp32, bf16 or fp16, one type a call; grads of that type or fp32; exp_avgs / exp_avg_sqs fp32; masters: fp32 copies of
+    16-bit parameters, which then carry the value (the parameter is written from them, rounded to nearest) -- without them an update
+    below half a unit in the last place of a 16-bit parameter is lost.  The i-th tensors of all lists have one shape and one dense
+    layout, whatever the order of their dimensions; sizes from zero.  No two written tensors may share memory.
+    step: 1 for the first step, or, like lr, a 0-dim fp32 device tensor read when the kernel runs (a captured step).
+    grad_scale: 0-dim fp32 device tensor the gradients are multiplied with on load (``grad_norm``)."""
+    _adamw("adamw_step", (params, grads, exp_avgs, exp_avg_sqs, None, None, masters), "wrwwssw", _ADAMW_NAMES, 32, step, lr, betas, eps,
+           weight_decay, grad_scale, 0)
+
+
+def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_roots, exp_avg_root_scales, *, step, lr, betas=(0.9, 0.999), eps=1e-8,
+                weight_decay=1e-2, grad_scale=None, masters=None, seed=0):
+    """``adamw_step`` with the states in 8 bits: exp_avgs (m) and exp_avg_roots (the ROOT of the second moment) are float8_e4m3fn
+    tensors, times one power of two (fp32 scales, ceil(n / 256) a tensor) for each 256 consecutive elements of memory; start from
+    zeros.  The step itself is computed in fp32 from the states' values; what is stored is rounded stochastically -- in the mean
+    exact, so that a change of 0.1 % a step is not lost -- with bits that depend on (seed, step, place in the lists) and nothing
+    else.  A root above zero never becomes zero; an element that is not finite becomes NaN and leaves its neighbours alone."""
+    _adamw("adamw8_step", (params, grads, exp_avgs, exp_avg_roots, exp_avg_scales, exp_avg_root_scales, masters), "wrwwssw", _ADAMW8_NAMES, 8,
+           step, lr, betas, eps, weight_decay, grad_scale, seed)
+
+
 # ---------------------------------------------------------------------------- glue
 def input_norm(x, eval_label, mean, std):
     b, cn, h, w = x.shape

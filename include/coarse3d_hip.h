@@ -323,6 +323,63 @@ int c3d_bias_from_partials(const float* partial, int n, int C, float* out, int a
 int c3d_sums_to_f32(const double* sums, int C, int col, float* out, int accumulate,
                     c3d_stream stream);
 
+/* ------------------------------------------------------------------ GroupNorm with an activation (channels last)
+ * Statistics of one sample and one group of channels: what takes BatchNorm2d's place (salsanext_proto.py:46,50, projector.py:20)
+ * when a GPU trains on one or two scans and batch statistics say little.  x is [N][HW][C] with C consecutive channels a pixel,
+ * `x_ps` elements from pixel to pixel and `x_ns` from sample to sample; y, dx are dense.  type: 0 fp32, 1 bf16, 2 fp16 (x, y, dy,
+ * dx alike); gamma, beta [C] fp32 (NULL: 1, 0).  act: 0 none, 1 LeakyReLU(slope), 2 SiLU.
+ *   mean, rstd [N][G] : of the HW * C / G values of (n, g), biased variance, rstd = 1 / sqrt(var + eps)
+ *   y = act((x - mean) * rstd * gamma + beta)
+ * ws: c3d_group_norm_ws_floats() floats.  N * HW == 0 is allowed (nothing to normalise).                            */
+int64_t c3d_group_norm_ws_floats(int N, int64_t HW, int C, int G, int type);
+int c3d_group_norm(const void* x, int64_t x_ns, int64_t x_ps, int N, int64_t HW, int C, int G, int type,
+                   const float* gamma, const float* beta, float eps, int act, float slope, void* y, float* mean,
+                   float* rstd, float* ws, c3d_stream stream);
+/* with dz = dy * act'(z), t = dz * gamma, xhat = (x - mean) * rstd and means over the values of (n, g):
+ *   dx = rstd * (t - mean(t) - xhat * mean(t * xhat)),  dgamma = sum dz * xhat,  dbeta = sum dz  (dgamma, dbeta may be NULL)
+ * The same ws.  Sums are folded in a fixed order: equal inputs give equal bits.                                      */
+int c3d_group_norm_bwd(const void* dy, int64_t dy_ns, int64_t dy_ps, const void* x, int64_t x_ns, int64_t x_ps, int N,
+                       int64_t HW, int C, int G, int type, const float* mean, const float* rstd, const float* gamma,
+                       const float* beta, int act, float slope, void* dx, float* dgamma, float* dbeta, float* ws,
+                       c3d_stream stream);
+
+/* ------------------------------------------------------------------ optimiser over many tensors
+ * AdamW as the reference steps it (trainer.py:146-151, torch.optim.AdamW), over a list of tensors in a few launches, with the
+ * moments in 32 bits or in 8; the global norm of the gradients and their clipping.  Lists are HOST arrays of this record (they
+ * travel as kernel arguments: nothing to copy, nothing to keep, capturable).                                        */
+typedef struct {
+  void* ptr[7];   /* 0 parameter, 1 gradient, 2 exp_avg, 3 exp_avg_sq (8 bits: its root), 4 / 5 block scales of 2 / 3 (8 bits),
+                     6 fp32 master copy of a 16-bit parameter; slots that a call does not use may be NULL           */
+  int64_t n;      /* elements; 0 is allowed                                                                        */
+} c3d_opt_tensor;
+/* elements that share one scale of an 8-bit state                                                                 */
+#define C3D_ADAMW8_BLOCK 256
+/* number of doubles of c3d_grad_norm's workspace (host call)                                                       */
+int64_t c3d_grad_norm_partials(const c3d_opt_tensor* t, int count);
+/* *norm = sqrt(sum of all squares) (sums in 64 bits, fixed order), *scale = min(1, max_norm / (norm + 1e-6)): the factor of
+ * torch.nn.utils.clip_grad_norm_, for c3d_scale_tensors or c3d_adamw_desc.grad_scale.  type as above.               */
+int c3d_grad_norm(const c3d_opt_tensor* t, int count, int type, double max_norm, double* partial, float* norm,
+                  float* scale, c3d_stream stream);
+/* gradient *= *scale, in place                                                                                     */
+int c3d_scale_tensors(const c3d_opt_tensor* t, int count, int type, const float* scale, c3d_stream stream);
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* grad_scale;   /* device scalar the gradients are multiplied with on load, or NULL                    */
+  const float* step_dev;     /* not NULL: the step count / the learning rate are read on the device when the kernel */
+  const float* lr_dev;       /*   runs (captured steps)                                                             */
+  int64_t step;              /* 1 for the first step                                                                */
+  int32_t param_type, grad_type, state_bits, has_master;
+  uint32_t seed;             /* 8 bits: of the stochastic rounding                                                  */
+  int32_t reserved;
+} c3d_adamw_desc;
+/* m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps).
+ * state_bits 8: m and sqrt(v) are e4m3 numbers times a power of two for each block of C3D_ADAMW8_BLOCK consecutive elements
+ * (the block's largest finite value lies in (224, 448] units), rounded stochastically with bits that depend on (seed, step, place
+ * in the list); sqrt(v) > 0 is never stored as 0; what is not finite is stored as NaN.                               */
+int c3d_adamw_step(const c3d_opt_tensor* t, int count, const c3d_adamw_desc* d, c3d_stream stream);
+/* out2 = sizeof(c3d_opt_tensor), sizeof(c3d_adamw_desc) (host call, as c3d_abi_sizes)                               */
+int c3d_opt_abi_sizes(int32_t* out2);
+
 /* ------------------------------------------------------------------ block glue (HBM-bound) */
 
 /* x = (x - mean[c]) / std[c] * (eval_label > 0)   NCHW  (trainer.py:599-609)                */

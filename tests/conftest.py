@@ -22,6 +22,7 @@ def pytest_configure(config):
 _NOT_ENGINE_PARITY = {
     "test_gpu_dp.py": None,                      # multi-process exchange infrastructure + bench.py subprocesses (the default run covers them)
     "test_gpu_projection.py": None, "test_gpu_knn.py": None, "test_gpu_weak_label.py": None, "test_gpu_metrics.py": None,
+    "test_gpu_group_norm.py": None, "test_gpu_adamw_many.py": None,             # never touch a matrix engine
     "test_gpu_bf16_oracle.py": None, "test_gpu_bf16_storage.py": None,          # pin the bf16 engine themselves
     "test_gpu_step.py": ("test_captured_step_survives_thousands", "test_launch_by_launch_steps_do_not_wait", "test_no_usage_mode_holds",
                          "test_graphed_inference_survives", "test_eval_forward_is_graph_capturable"),
