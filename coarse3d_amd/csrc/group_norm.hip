@@ -6,15 +6,17 @@
 //     dbeta = sum dz,  dgamma = sum dz * xhat  (over samples and pixels),  dx = rstd * (t - mean(t) - xhat * mean(t * xhat)).
 //
 // A thread owns V consecutive channels (16 bytes where alignment allows) and walks pixels, so that every load is a whole vector of
-// a pixel's row whatever D is; what belongs to a group is only put together when the per-channel partial sums are folded.
+// a pixel's row whatever D is.  Two forms:
+//   small: one workgroup holds all values of a (sample, group) in registers -- one launch, one read, no workspace;
+//   large: a pass for the statistics, a pass that applies them.  The second walks the tensor backwards, so that it begins with what
+//          the first has left in the caches, and its workgroups fold the partial statistics of their sample by themselves.
+#include <algorithm>
 #include <initializer_list>
 #include <type_traits>
 #include "common.h"
 #include "../../include/coarse3d_hip.h"
 
 namespace {
-
-constexpr int kThreads = 256;
 
 enum { ACT_NONE = 0, ACT_LRELU = 1, ACT_SILU = 2 };
 
@@ -52,310 +54,632 @@ __device__ __forceinline__ float act_bwd(float z, float slope) {
   return 1.f;
 }
 
-// How an image is cut: `qt` vectors (of Q = C / V) a workgroup, `pl` pixels side by side, `nb` workgroups along a sample's pixels
-struct Plan {
-  int Q, qt, pl, tiles, nb;
-  int64_t ppb;              // pixels a workgroup
-};
-inline Plan make_plan(int N, int64_t HW, int C, int V) {
-  Plan p;
-  p.Q = C / V;
-  p.qt = p.Q < kThreads ? p.Q : kThreads;
-  p.tiles = (p.Q + p.qt - 1) / p.qt;
-  p.pl = kThreads / p.qt;
-  const int64_t most = (HW + p.pl * 8 - 1) / (p.pl * 8);       // at least eight pixels a thread
-  int64_t want = 1024 / ((int64_t)N * p.tiles);
-  if (want < 1) want = 1;
-  if (want > 512) want = 512;
-  p.nb = (int)(most < want ? most : want);
-  if (p.nb < 1) p.nb = 1;
-  p.ppb = (HW + p.nb - 1) / p.nb;
-  return p;
-}
-
 struct Img {
   int64_t ns, ps;           // elements from sample to sample and from pixel to pixel
 };
 
-// per workgroup and channel: mean and sum of squared deviations of its pixels, [2][N][nb][C].  Values are shifted by the chunk's first
-// pixel, so that a mean far from zero costs nothing.
+// ---------------------------------------------------------------- small: a (sample, group) in one workgroup
+
+template <int V>
+constexpr int kSmallThreads = V == 8 ? 512 : 1024;
+template <int V>
+constexpr int kSmallVecs = V == 8 ? 4 : 16 / V;        // vectors a thread holds
+// thread t: vector t % dv of the group's D / V, pixels t / dv + r * pl
+
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = c3d_wave_sum(v);
+  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[w] = v;
+  __syncthreads();
+  float s = 0.f;
+  for (int i = 0; i < nw; ++i) s += red[i];
+  return s;
+}
+
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kSmallThreads<V>) void gn_small_kernel(const T* __restrict__ x, Img xi, int HW, int C, int G, int dv, int pl,
+                                                                  const float* __restrict__ gamma, const float* __restrict__ beta, float eps,
+                                                                  float slope, T* __restrict__ y, float* __restrict__ mean,
+                                                                  float* __restrict__ rstd) {
+  constexpr int R = kSmallVecs<V>;
+  __shared__ float red[16];
+  const int n = blockIdx.x / G, g = blockIdx.x % G, l = threadIdx.x / dv, c = g * (C / G) + (threadIdx.x % dv) * V;
+  const T* xs = x + n * xi.ns + c;
+  Vec<T, V> raw[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (l < pl && l + r * pl < HW) raw[r] = *reinterpret_cast<const Vec<T, V>*>(xs + (int64_t)(l + r * pl) * xi.ps);
+  const float count = (float)HW * (float)(C / G);
+  float s = 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (l < pl && l + r * pl < HW)
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += (float)raw[r].v[e];
+  const float mu = block_sum(s, red) / count;
+  s = 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (l < pl && l + r * pl < HW)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = (float)raw[r].v[e] - mu;
+        s = fmaf(d, d, s);
+      }
+  const float rs = 1.f / sqrtf(block_sum(s, red) / count + eps);
+  if (threadIdx.x == 0) {
+    mean[blockIdx.x] = mu;
+    rstd[blockIdx.x] = rs;
+  }
+  if (l >= pl) return;
+  float ga[V], be[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    ga[e] = gamma ? gamma[c + e] : 1.f;
+    be[e] = beta ? beta[c + e] : 0.f;
+  }
+  T* ys = y + (int64_t)n * HW * C + c;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (l + r * pl < HW) {
+      float o[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = act_fwd<ACT>(fmaf(((float)raw[r].v[e] - mu) * rs, ga[e], be[e]), slope);
+      stv<T, V>(ys + (int64_t)(l + r * pl) * C, o);
+    }
+}
+
+// chan: [N][C] pairs (sum dz, sum dz xhat) of a sample, or with N == 1 straight into dbeta, dgamma
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kSmallThreads<V>) void gn_small_bwd_kernel(const T* __restrict__ dy, Img di, const T* __restrict__ x, Img xi, int HW, int C,
+                                                                      int G, int dv, int pl, const float* __restrict__ mean,
+                                                                      const float* __restrict__ rstd, const float* __restrict__ gamma,
+                                                                      const float* __restrict__ beta, float slope, T* __restrict__ dx,
+                                                                      float2* __restrict__ chan, float* __restrict__ dgamma,
+                                                                      float* __restrict__ dbeta) {
+  constexpr int R = kSmallVecs<V>;
+  extern __shared__ float2 rows[];                       // [pl][D], then [pl / 8][D]
+  __shared__ float red[16];
+  const int n = blockIdx.x / G, g = blockIdx.x % G, D = C / G, l = threadIdx.x / dv, q = threadIdx.x % dv, c = g * D + q * V;
+  const T* xs = x + n * xi.ns + c;
+  const T* ds = dy + n * di.ns + c;
+  Vec<T, V> xr[R], dr[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (l < pl && l + r * pl < HW) {
+      xr[r] = *reinterpret_cast<const Vec<T, V>*>(xs + (int64_t)(l + r * pl) * xi.ps);
+      dr[r] = *reinterpret_cast<const Vec<T, V>*>(ds + (int64_t)(l + r * pl) * di.ps);
+    }
+  const float mu = mean[blockIdx.x], rs = rstd[blockIdx.x];
+  float ga[V], be[V], a[V], b[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    ga[e] = l < pl && gamma ? gamma[c + e] : 1.f;
+    be[e] = l < pl && beta ? beta[c + e] : 0.f;
+    a[e] = b[e] = 0.f;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (l < pl && l + r * pl < HW)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float xh = ((float)xr[r].v[e] - mu) * rs;
+        const float dz = (float)dr[r].v[e] * act_bwd<ACT>(fmaf(xh, ga[e], be[e]), slope);
+        a[e] += dz;
+        b[e] = fmaf(dz, xh, b[e]);
+      }
+  float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    s1 = fmaf(a[e], ga[e], s1);
+    s2 = fmaf(b[e], ga[e], s2);
+  }
+  const float count = (float)HW * (float)D;
+  const float c1 = block_sum(s1, red) / count, c2 = block_sum(s2, red) / count;
+  if (l < pl) {
+    T* os = dx + (int64_t)n * HW * C + c;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (l + r * pl < HW) {
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float xh = ((float)xr[r].v[e] - mu) * rs;
+          const float t = (float)dr[r].v[e] * act_bwd<ACT>(fmaf(xh, ga[e], be[e]), slope) * ga[e];
+          o[e] = rs * (t - c1 - xh * c2);
+        }
+        stv<T, V>(os + (int64_t)(l + r * pl) * C, o);
+      }
+  }
+  if (!chan) return;
+  // the channels' sums: eight rows to one until one is left
+  if (l < pl)
+#pragma unroll
+    for (int e = 0; e < V; ++e) rows[l * D + q * V + e] = make_float2(a[e], b[e]);
+  float2* from = rows;
+  float2* to = rows + pl * D;
+  for (int k = pl; k > 1; k = (k + 7) / 8) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < (k + 7) / 8 * D; i += blockDim.x) {
+      const int row = i / D, ch = i % D;
+      float2 v = make_float2(0.f, 0.f);
+      for (int j = row * 8; j < row * 8 + 8 && j < k; ++j) {
+        v.x += from[j * D + ch].x;
+        v.y += from[j * D + ch].y;
+      }
+      to[i] = v;
+    }
+    float2* t = from;
+    from = to;
+    to = t;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < D; i += blockDim.x) {
+    if (gridDim.x == (unsigned)G) {
+      if (dbeta) dbeta[g * D + i] = from[i].x;
+      if (dgamma) dgamma[g * D + i] = from[i].y;
+    } else {
+      chan[(int64_t)n * C + g * D + i] = from[i];
+    }
+  }
+}
+
+// ---------------------------------------------------------------- large: two passes
+
+// How an image is cut.  A tile of channels is `gpt` whole groups (split == 1), or one of `split` parts of a group too wide for a
+// workgroup; qt vectors wide, `pl` pixels side by side.  A sample's pixels are cut into nb chunks of ppb.
+struct Plan {
+  int D, qt, pl, threads, tiles, gpt, split, nb;
+  int64_t ppb;
+};
+struct Tile {
+  int c0, nq, g0, ng, part;      // first channel, vectors, first group, groups, part of the group
+};
+template <int V>
+__device__ __forceinline__ Tile tile_of(const Plan& p, int t, int G) {
+  Tile r;
+  if (p.split == 1) {
+    r.g0 = t * p.gpt;
+    r.ng = min(p.gpt, G - r.g0);
+    r.c0 = r.g0 * p.D;
+    r.nq = r.ng * p.D / V;
+    r.part = 0;
+  } else {
+    r.g0 = t / p.split;
+    r.ng = 1;
+    r.part = t % p.split;
+    r.c0 = r.g0 * p.D + r.part * p.qt * V;
+    r.nq = min(p.qt, p.D / V - r.part * p.qt);
+  }
+  return r;
+}
+// the second pass begins where the first ended, workgroup by workgroup on the same XCD (block b runs on XCD b % 8)
+__device__ __forceinline__ int backwards(int b, int n) {
+  const int whole = n & ~7;
+  return b < whole ? whole - 8 - (b & ~7) + (b & 7) : b;
+}
+
+// sums of a pair over the 16 lanes of a DPP row, in 64 bits
+__device__ __forceinline__ void sum16(double& a, double& b) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    a += __shfl_xor(a, o, 64);
+    b += __shfl_xor(b, o, 64);
+  }
+}
+
+// Partial results: [N][G][nb][split] pairs, part_at() the first of a chunk
+__device__ __forceinline__ int64_t part_at(const Plan& p, int G, int n, int g) { return ((int64_t)n * G + g) * p.nb * p.split; }
+
+// unrolled walk over a chunk's pixels: U loads in flight ahead of their use
+template <int U, class F, class H>
+__device__ __forceinline__ void walk(int64_t i, int64_t end, int step, F load, H use) {
+  for (; i + (int64_t)(U - 1) * step < end; i += (int64_t)U * step) {
+    decltype(load(i)) r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) r[u] = load(i + (int64_t)u * step);
+#pragma unroll
+    for (int u = 0; u < U; ++u) use(i + (int64_t)u * step, r[u]);
+  }
+  for (; i < end; i += step) use(i, load(i));
+}
+
+// sums of s1, s2 [V] over the workgroup's `pl` pixel lanes: -> shared sum[ch] of the tile's channels
+template <int V>
+__device__ __forceinline__ void join_lanes(const Plan& p, const Tile& t, bool on, int l, int q, const float (&s1)[V], const float (&s2)[V], float2* sum) {
+  const int W = p.qt * V, wt = t.nq * V;
+  if (on)
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[l * W + q * V + e] = make_float2(s1[e], s2[e]);
+  // halves onto halves: a few barriers instead of one thread's walk over all lanes
+  for (int k = p.pl; k > 1;) {
+    const int h = (k + 1) / 2;
+    __syncthreads();
+    for (int i = threadIdx.x; i < (k - h) * W; i += blockDim.x) {
+      if (i % W < wt) {
+        const float2 o = sum[h * W + i];
+        sum[i].x += o.x;
+        sum[i].y += o.y;
+      }
+    }
+    k = h;
+  }
+  __syncthreads();
+}
+
+// First pass: mean and sum of squared deviations of every group in the chunk.  Values are shifted by the chunk's first pixel, so that
+// a mean far from zero costs nothing.
 template <class T, int V>
-__global__ __launch_bounds__(kThreads) void gn_stats_kernel(const T* __restrict__ x, Img xi, Plan p, int N, int64_t HW, int C,
-                                                           float* __restrict__ part) {
-  extern __shared__ float red[];
-  const int tile = blockIdx.x % p.tiles, b = (blockIdx.x / p.tiles) % p.nb, n = blockIdx.x / (p.tiles * p.nb);
-  const int l = threadIdx.x / p.qt, q = tile * p.qt + threadIdx.x % p.qt;
-  const bool on = l < p.pl && q < p.Q;
+__global__ __launch_bounds__(512) void gn_stats_kernel(const T* __restrict__ x, Img xi, Plan p, int64_t HW, int G, float2* __restrict__ part) {
+  extern __shared__ float2 sum[];
+  const Tile t = tile_of<V>(p, blockIdx.x % p.tiles, G);
+  const int b = (blockIdx.x / p.tiles) % p.nb, n = blockIdx.x / (p.tiles * p.nb);
+  const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
+  const bool on = l < p.pl && q < t.nq;
   const int64_t p0 = b * p.ppb, p1 = p0 + p.ppb < HW ? p0 + p.ppb : HW;
-  const T* xs = x + n * xi.ns + (int64_t)q * V;
   float shift[V], s1[V], s2[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) shift[e] = s1[e] = s2[e] = 0.f;
-  if (on && p0 < p1) {
+  if (on) {
+    const T* xs = x + n * xi.ns + t.c0 + q * V;
     ldv<T, V>(xs + p0 * xi.ps, shift);
-    for (int64_t i = p0 + l; i < p1; i += p.pl) {
-      float r[V];
-      ldv<T, V>(xs + i * xi.ps, r);
+    walk<8>(p0 + l, p1, p.pl, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); },
+            [&](int64_t, const Vec<T, V>& r) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = r[e] - shift[e];
-        s1[e] += d;
-        s2[e] = fmaf(d, d, s2[e]);
+              for (int e = 0; e < V; ++e) {
+                const float d = (float)r.v[e] - shift[e];
+                s1[e] += d;
+                s2[e] = fmaf(d, d, s2[e]);
+              }
+            });
+  }
+  join_lanes<V>(p, t, on, l, q, s1, s2, sum);
+  const float cnt = (float)(p1 - p0);
+  float2* shifts = sum + p.qt * V;                        // (row 1: free again)
+  if (on && l == 0)
+#pragma unroll
+    for (int e = 0; e < V; ++e) shifts[q * V + e].x = shift[e];
+  __syncthreads();
+  // sixteen lanes a group: mean and deviations over its channels
+  const int chans = p.split == 1 ? p.D : t.nq * V;
+  for (int g = threadIdx.x / 16; g < (t.ng + 3) / 4 * 4; g += blockDim.x / 16) {
+    double m = 0.0, m2 = 0.0;
+    if (g < t.ng)
+      for (int k = threadIdx.x % 16; k < chans; k += 16) {
+        const float2 v = sum[g * p.D + k];
+        const double d = (double)v.x / cnt, mu = (double)shifts[g * p.D + k].x + d;
+        m += mu;
+        m2 += ((double)v.y - (double)v.x * d) + cnt * mu * mu;
       }
+    sum16(m, m2);
+    if (g < t.ng && threadIdx.x % 16 == 0) {
+      const double mu = m / chans;
+      part[part_at(p, G, n, t.g0 + g) + b * p.split + t.part] = make_float2((float)mu, (float)fmax(m2 - cnt * chans * mu * mu, 0.0));
     }
   }
-  const int W = p.qt * V;
-  if (on) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      red[(l * 2 + 0) * W + (threadIdx.x % p.qt) * V + e] = s1[e];
-      red[(l * 2 + 1) * W + (threadIdx.x % p.qt) * V + e] = s2[e];
+}
+
+// mean and rstd of (n, g) from its partial results, by sixteen lanes; every lane gets them
+__device__ __forceinline__ float2 fold_stats(const float2* __restrict__ part, const Plan& p, int V, int64_t HW, int G, int n, int g, float eps) {
+  const float2* a = part + part_at(p, G, n, g);
+  double s = 0.0, s2 = 0.0;
+  for (int i = threadIdx.x % 16; i < p.nb * p.split; i += 16) {
+    const int b = i / p.split, k = i % p.split;
+    const int64_t p0 = b * p.ppb, p1 = p0 + p.ppb < HW ? p0 + p.ppb : HW;
+    const double cnt = (double)(p1 - p0) * (p.split == 1 ? p.D : min(p.qt * V, p.D - k * p.qt * V));
+    const float2 v = a[i];
+    s += cnt * v.x;
+    s2 += (double)v.y + cnt * ((double)v.x * v.x);
+  }
+  sum16(s, s2);
+  const double M = (double)HW * p.D, mu = s / M, var = s2 / M - mu * mu;
+  return make_float2((float)mu, (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)eps)));
+}
+
+template <int V>
+__global__ __launch_bounds__(64) void gn_fold_kernel(const float2* __restrict__ part, Plan p, int64_t HW, int N, int G, float eps, float* __restrict__ mean,
+                                                    float* __restrict__ rstd) {
+  const int i = blockIdx.x * 4 + threadIdx.x / 16;
+  const int k = min(i, N * G - 1);
+  const float2 r = fold_stats(part, p, V, HW, G, k / G, k % G, eps);
+  if (i < N * G && threadIdx.x % 16 == 0) {
+    mean[i] = r.x;
+    rstd[i] = r.y;
+  }
+}
+
+// Second pass.  part != NULL: the statistics are still in pieces; every workgroup folds those of its groups
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(512) void gn_apply_kernel(const T* __restrict__ x, Img xi, Plan p, int64_t HW, int C, int G, const float2* __restrict__ part,
+                                                      float eps, float* __restrict__ mean, float* __restrict__ rstd,
+                                                      const float* __restrict__ gamma, const float* __restrict__ beta, float slope,
+                                                      T* __restrict__ y) {
+  extern __shared__ float2 stat[];                       // [gpt]
+  const int block = backwards(blockIdx.x, gridDim.x);
+  const Tile t = tile_of<V>(p, block % p.tiles, G);
+  const int b = (block / p.tiles) % p.nb, n = block / (p.tiles * p.nb);
+  for (int g = threadIdx.x / 16; g < (t.ng + 3) / 4 * 4; g += blockDim.x / 16) {
+    const int k = n * G + t.g0 + min(g, t.ng - 1);
+    const float2 r = part ? fold_stats(part, p, V, HW, G, n, k - n * G, eps) : make_float2(mean[k], rstd[k]);
+    if (g < t.ng && threadIdx.x % 16 == 0) {
+      stat[g] = r;
+      if (part && b == 0 && t.part == 0) {
+        mean[k] = r.x;
+        rstd[k] = r.y;
+      }
     }
   }
   __syncthreads();
-  if (on && l == 0) {
-    const float cnt = (float)(p1 - p0);
-    float* o = part + ((int64_t)n * p.nb + b) * C + (int64_t)q * V;
-    const int64_t plane = (int64_t)N * p.nb * C;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float a1 = 0.f, a2 = 0.f;
-      for (int k = 0; k < p.pl; ++k) {
-        a1 += red[(k * 2 + 0) * W + threadIdx.x * V + e];
-        a2 += red[(k * 2 + 1) * W + threadIdx.x * V + e];
-      }
-      const bool any = p1 > p0;
-      const float mu = any ? a1 / cnt : 0.f;
-      o[e] = shift[e] + mu;
-      o[plane + e] = any ? a2 - a1 * mu : 0.f;
-    }
-  }
-}
-
-// one workgroup a (sample, group): joins the partial means and squared deviations in 64 bits
-__global__ __launch_bounds__(kThreads) void gn_fold_kernel(const float* __restrict__ part, Plan p, int N, int64_t HW, int C, int G, float eps,
-                                                          float* __restrict__ mean, float* __restrict__ rstd) {
-  __shared__ double red[4];
-  const int n = blockIdx.x / G, g = blockIdx.x % G, D = C / G;
-  const int64_t plane = (int64_t)N * p.nb * C;
-  const float* a = part + (int64_t)n * p.nb * C + g * D;
-  const double M = (double)HW * D;
-  const int total = p.nb * D;
-  auto block_sum = [&](double s) {
-    s = c3d_wave_sum_d(s);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-    __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
-  };
-  auto count = [&](int b) {
-    const int64_t p0 = b * p.ppb, p1 = p0 + p.ppb < HW ? p0 + p.ppb : HW;
-    return p1 > p0 ? (double)(p1 - p0) : 0.0;
-  };
-  double s = 0.0;
-  for (int i = threadIdx.x; i < total; i += kThreads) s += count(i / D) * (double)a[(int64_t)(i / D) * C + i % D];
-  const double mu = block_sum(s) / M;
-  s = 0.0;
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const int64_t at = (int64_t)(i / D) * C + i % D;
-    const double d = (double)a[at] - mu;
-    s += (double)a[plane + at] + count(i / D) * d * d;
-  }
-  const double var = block_sum(s) / M;
-  if (threadIdx.x == 0) {
-    mean[blockIdx.x] = (float)mu;
-    rstd[blockIdx.x] = (float)(1.0 / sqrt(var + (double)eps));
-  }
-}
-
-template <class T, int V, int ACT>
-__global__ __launch_bounds__(kThreads) void gn_apply_kernel(const T* __restrict__ x, Img xi, Plan p, int64_t HW, int C, int G,
-                                                           const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                           const float* __restrict__ gamma, const float* __restrict__ beta, float slope,
-                                                           T* __restrict__ y) {
-  const int tile = blockIdx.x % p.tiles, b = (blockIdx.x / p.tiles) % p.nb, n = blockIdx.x / (p.tiles * p.nb);
-  const int l = threadIdx.x / p.qt, q = tile * p.qt + threadIdx.x % p.qt;
-  if (l >= p.pl || q >= p.Q) return;
+  const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
+  if (l >= p.pl || q >= t.nq) return;
   const int64_t p0 = b * p.ppb, p1 = p0 + p.ppb < HW ? p0 + p.ppb : HW;
-  const T* xs = x + n * xi.ns + (int64_t)q * V;
-  T* ys = y + (int64_t)n * HW * C + (int64_t)q * V;
-  float mu[V], sc[V], sh[V];
+  const T* xs = x + n * xi.ns + t.c0 + q * V;
+  T* ys = y + (int64_t)n * HW * C + t.c0 + q * V;
+  float mu[V], rs[V], ga[V], be[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const int c = q * V + e, g = n * G + c / (C / G);
-    mu[e] = mean[g];
-    sc[e] = rstd[g] * (gamma ? gamma[c] : 1.f);
-    sh[e] = beta ? beta[c] : 0.f;
+    const int c = t.c0 + q * V + e;
+    const float2 v = stat[p.split == 1 ? (q * V + e) / p.D : 0];
+    mu[e] = v.x;
+    rs[e] = v.y;
+    ga[e] = gamma ? gamma[c] : 1.f;
+    be[e] = beta ? beta[c] : 0.f;
   }
-  for (int64_t i = p0 + l; i < p1; i += p.pl) {
-    float r[V];
-    ldv<T, V>(xs + i * xi.ps, r);
+  walk<4>(p0 + l, p1, p.pl, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); },
+          [&](int64_t i, const Vec<T, V>& r) {
+            float o[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) r[e] = act_fwd<ACT>(fmaf(r[e] - mu[e], sc[e], sh[e]), slope);
-    stv<T, V>(ys + i * C, r);
-  }
+            for (int e = 0; e < V; ++e) o[e] = act_fwd<ACT>(fmaf(((float)r.v[e] - mu[e]) * rs[e], ga[e], be[e]), slope);
+            stv<T, V>(ys + i * C, o);
+          });
 }
 
-// per workgroup and channel: sum dz and sum dz * xhat, [2][N][nb][C]
+template <class T, int V>
+struct Two {
+  Vec<T, V> x, d;
+};
+
+// Backward, first pass: per chunk and group (sum t, sum t xhat) -> part, and per channel (sum dz, sum dz xhat) -> chan [N][nb][C]
 template <class T, int V, int ACT>
-__global__ __launch_bounds__(kThreads) void gn_bwd_stats_kernel(const T* __restrict__ dy, Img di, const T* __restrict__ x, Img xi, Plan p, int N,
-                                                               int64_t HW, int C, int G, const float* __restrict__ mean,
-                                                               const float* __restrict__ rstd, const float* __restrict__ gamma,
-                                                               const float* __restrict__ beta, float slope, float* __restrict__ part) {
-  extern __shared__ float red[];
-  const int tile = blockIdx.x % p.tiles, b = (blockIdx.x / p.tiles) % p.nb, n = blockIdx.x / (p.tiles * p.nb);
-  const int l = threadIdx.x / p.qt, q = tile * p.qt + threadIdx.x % p.qt;
-  const bool on = l < p.pl && q < p.Q;
+__global__ __launch_bounds__(512) void gn_bwd_stats_kernel(const T* __restrict__ dy, Img di, const T* __restrict__ x, Img xi, Plan p, int64_t HW, int C,
+                                                          int G, const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                          const float* __restrict__ gamma, const float* __restrict__ beta, float slope,
+                                                          float2* __restrict__ part, float2* __restrict__ chan) {
+  extern __shared__ float2 sum[];
+  const Tile t = tile_of<V>(p, blockIdx.x % p.tiles, G);
+  const int b = (blockIdx.x / p.tiles) % p.nb, n = blockIdx.x / (p.tiles * p.nb);
+  const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
+  const bool on = l < p.pl && q < t.nq;
   const int64_t p0 = b * p.ppb, p1 = p0 + p.ppb < HW ? p0 + p.ppb : HW;
   float s1[V], s2[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
   if (on) {
-    const T* xs = x + n * xi.ns + (int64_t)q * V;
-    const T* ds = dy + n * di.ns + (int64_t)q * V;
+    const T* xs = x + n * xi.ns + t.c0 + q * V;
+    const T* ds = dy + n * di.ns + t.c0 + q * V;
     float mu[V], rs[V], ga[V], be[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = q * V + e, g = n * G + c / (C / G);
-      mu[e] = mean[g];
-      rs[e] = rstd[g];
+      const int c = t.c0 + q * V + e, k = n * G + t.g0 + (p.split == 1 ? (q * V + e) / p.D : 0);
+      mu[e] = mean[k];
+      rs[e] = rstd[k];
       ga[e] = gamma ? gamma[c] : 1.f;
       be[e] = beta ? beta[c] : 0.f;
     }
-    for (int64_t i = p0 + l; i < p1; i += p.pl) {
-      float r[V], d[V];
-      ldv<T, V>(xs + i * xi.ps, r);
-      ldv<T, V>(ds + i * di.ps, d);
+    walk<4>(p0 + l, p1, p.pl,
+            [&](int64_t i) {
+              return Two<T, V>{*reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps), *reinterpret_cast<const Vec<T, V>*>(ds + i * di.ps)};
+            },
+            [&](int64_t, const Two<T, V>& r) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float xh = (r[e] - mu[e]) * rs[e];
-        const float dz = d[e] * act_bwd<ACT>(fmaf(xh, ga[e], be[e]), slope);
-        s1[e] += dz;
-        s2[e] = fmaf(dz, xh, s2[e]);
-      }
-    }
+              for (int e = 0; e < V; ++e) {
+                const float xh = ((float)r.x.v[e] - mu[e]) * rs[e];
+                const float dz = (float)r.d.v[e] * act_bwd<ACT>(fmaf(xh, ga[e], be[e]), slope);
+                s1[e] += dz;
+                s2[e] = fmaf(dz, xh, s2[e]);
+              }
+            });
   }
-  const int W = p.qt * V;
-  if (on) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      red[(l * 2 + 0) * W + (threadIdx.x % p.qt) * V + e] = s1[e];
-      red[(l * 2 + 1) * W + (threadIdx.x % p.qt) * V + e] = s2[e];
-    }
-  }
-  __syncthreads();
-  if (on && l == 0) {
-    float* o = part + ((int64_t)n * p.nb + b) * C + (int64_t)q * V;
-    const int64_t plane = (int64_t)N * p.nb * C;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float a1 = 0.f, a2 = 0.f;
-      for (int k = 0; k < p.pl; ++k) {
-        a1 += red[(k * 2 + 0) * W + threadIdx.x * V + e];
-        a2 += red[(k * 2 + 1) * W + threadIdx.x * V + e];
+  join_lanes<V>(p, t, on, l, q, s1, s2, sum);
+  if (chan)
+    for (int i = threadIdx.x; i < t.nq * V; i += blockDim.x) chan[((int64_t)n * p.nb + b) * C + t.c0 + i] = sum[i];
+  const int chans = p.split == 1 ? p.D : t.nq * V;
+  for (int g = threadIdx.x / 16; g < (t.ng + 3) / 4 * 4; g += blockDim.x / 16) {
+    double a = 0.0, c = 0.0;
+    if (g < t.ng)
+      for (int k = threadIdx.x % 16; k < chans; k += 16) {
+        const float2 v = sum[g * p.D + k];
+        const double ga = gamma ? (double)gamma[t.c0 + g * p.D + k] : 1.0;
+        a += ga * v.x;
+        c += ga * v.y;
       }
-      o[e] = a1;
-      o[plane + e] = a2;
-    }
+    sum16(a, c);
+    if (g < t.ng && threadIdx.x % 16 == 0) part[part_at(p, G, n, t.g0 + g) + b * p.split + t.part] = make_float2((float)a, (float)c);
   }
 }
 
-// workgroups [0, N G): mean(t) and mean(t xhat) of a (sample, group) -> coef [2][N][G]; the rest: dgamma, dbeta of one channel each
-__global__ __launch_bounds__(kThreads) void gn_bwd_fold_kernel(const float* __restrict__ part, Plan p, int N, int64_t HW, int C, int G,
-                                                              const float* __restrict__ gamma, float* __restrict__ coef,
-                                                              float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  __shared__ double red[2][4];
-  const int D = C / G;
-  const int64_t plane = (int64_t)N * p.nb * C;
-  double s1 = 0.0, s2 = 0.0;
-  const bool group = blockIdx.x < (unsigned)(N * G);
-  if (group) {
-    const int n = blockIdx.x / G, g = blockIdx.x % G;
-    const float* a = part + (int64_t)n * p.nb * C + g * D;
-    for (int i = threadIdx.x; i < p.nb * D; i += kThreads) {
-      const int64_t at = (int64_t)(i / D) * C + i % D;
-      const double ga = gamma ? (double)gamma[g * D + i % D] : 1.0;
-      s1 += ga * (double)a[at];
-      s2 += ga * (double)a[plane + at];
-    }
-  } else {
-    const int c = blockIdx.x - N * G;
-    for (int i = threadIdx.x; i < N * p.nb; i += kThreads) {
-      s1 += (double)part[(int64_t)i * C + c];
-      s2 += (double)part[plane + (int64_t)i * C + c];
-    }
+// the means of t and t xhat over (n, g), by sixteen lanes
+__device__ __forceinline__ float2 fold_means(const float2* __restrict__ part, const Plan& p, int64_t HW, int G, int n, int g) {
+  const float2* a = part + part_at(p, G, n, g);
+  double s = 0.0, s2 = 0.0;
+  for (int i = threadIdx.x % 16; i < p.nb * p.split; i += 16) {
+    s += (double)a[i].x;
+    s2 += (double)a[i].y;
   }
-  s1 = c3d_wave_sum_d(s1);
-  s2 = c3d_wave_sum_d(s2);
-  if ((threadIdx.x & 63) == 0) {
-    red[0][threadIdx.x >> 6] = s1;
-    red[1][threadIdx.x >> 6] = s2;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    s1 = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
-    s2 = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    if (group) {
-      const double M = (double)HW * D;
-      coef[blockIdx.x] = (float)(s1 / M);
-      coef[N * G + blockIdx.x] = (float)(s2 / M);
-    } else {
-      const int c = blockIdx.x - N * G;
-      if (dbeta) dbeta[c] = (float)s1;
-      if (dgamma) dgamma[c] = (float)s2;
-    }
-  }
+  sum16(s, s2);
+  const double M = (double)HW * p.D;
+  return make_float2((float)(s / M), (float)(s2 / M));
+}
+__global__ __launch_bounds__(64) void gn_bwd_fold_kernel(const float2* __restrict__ part, Plan p, int64_t HW, int N, int G, float2* __restrict__ coef) {
+  const int i = blockIdx.x * 4 + threadIdx.x / 16;
+  const int k = min(i, N * G - 1);
+  const float2 r = fold_means(part, p, HW, G, k / G, k % G);
+  if (i < N * G && threadIdx.x % 16 == 0) coef[i] = r;
 }
 
+// dgamma, dbeta of 16 channels: the rows of chan [rows][C], in 64 bits and a fixed order
+__device__ __forceinline__ void fold_channels(const float2* __restrict__ chan, int64_t rows, int C, int c0, float* __restrict__ dgamma,
+                                              float* __restrict__ dbeta, double2* red) {
+  const int c = c0 + (threadIdx.x & 15), lanes = blockDim.x / 16;
+  double a = 0.0, b = 0.0;
+  if (c < C)
+#pragma unroll 4
+    for (int64_t r = threadIdx.x / 16; r < rows; r += lanes) {
+      const float2 v = chan[r * C + c];
+      a += (double)v.x;
+      b += (double)v.y;
+    }
+  a += __shfl_xor(a, 16, 64);
+  b += __shfl_xor(b, 16, 64);
+  a += __shfl_xor(a, 32, 64);
+  b += __shfl_xor(b, 32, 64);
+  if ((threadIdx.x & 63) < 16) red[(threadIdx.x >> 6) * 16 + (threadIdx.x & 15)] = make_double2(a, b);
+  __syncthreads();
+  if (threadIdx.x < 16 && c < C) {
+    a = b = 0.0;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
+      a += red[w * 16 + threadIdx.x].x;
+      b += red[w * 16 + threadIdx.x].y;
+    }
+    if (dbeta) dbeta[c] = (float)a;
+    if (dgamma) dgamma[c] = (float)b;
+  }
+}
+__global__ __launch_bounds__(256) void gn_channels_kernel(const float2* __restrict__ chan, int64_t rows, int C, float* __restrict__ dgamma,
+                                                         float* __restrict__ dbeta) {
+  __shared__ double2 red[8 * 16];
+  fold_channels(chan, rows, C, blockIdx.x * 16, dgamma, dbeta, red);
+}
+
+// Backward, second pass.  The first `extra` workgroups fold dgamma and dbeta; folded: part holds [N][G] means already
 template <class T, int V, int ACT>
-__global__ __launch_bounds__(kThreads) void gn_bwd_apply_kernel(const T* __restrict__ dy, Img di, const T* __restrict__ x, Img xi, Plan p, int N,
-                                                               int64_t HW, int C, int G, const float* __restrict__ mean,
-                                                               const float* __restrict__ rstd, const float* __restrict__ gamma,
-                                                               const float* __restrict__ beta, float slope, const float* __restrict__ coef,
-                                                               T* __restrict__ dx) {
-  const int tile = blockIdx.x % p.tiles, b = (blockIdx.x / p.tiles) % p.nb, n = blockIdx.x / (p.tiles * p.nb);
-  const int l = threadIdx.x / p.qt, q = tile * p.qt + threadIdx.x % p.qt;
-  if (l >= p.pl || q >= p.Q) return;
+__global__ __launch_bounds__(512) void gn_bwd_apply_kernel(const T* __restrict__ dy, Img di, const T* __restrict__ x, Img xi, Plan p, int64_t HW, int N,
+                                                          int C, int G, const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                          const float* __restrict__ gamma, const float* __restrict__ beta, float slope,
+                                                          const float2* __restrict__ part, int folded, const float2* __restrict__ chan, int extra,
+                                                          float* __restrict__ dgamma, float* __restrict__ dbeta, T* __restrict__ dx) {
+  extern __shared__ float2 stat[];
+  if ((int)blockIdx.x < extra) {
+    fold_channels(chan, (int64_t)N * p.nb, C, blockIdx.x * 16, dgamma, dbeta, reinterpret_cast<double2*>(stat));
+    return;
+  }
+  const int block = backwards(blockIdx.x - extra, gridDim.x - extra);
+  const Tile t = tile_of<V>(p, block % p.tiles, G);
+  const int b = (block / p.tiles) % p.nb, n = block / (p.tiles * p.nb);
+  for (int g = threadIdx.x / 16; g < (t.ng + 3) / 4 * 4; g += blockDim.x / 16) {
+    const int k = t.g0 + min(g, t.ng - 1);
+    const float2 r = folded ? part[n * G + k] : fold_means(part, p, HW, G, n, k);
+    if (g < t.ng && threadIdx.x % 16 == 0) stat[g] = r;
+  }
+  __syncthreads();
+  const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
+  if (l >= p.pl || q >= t.nq) return;
   const int64_t p0 = b * p.ppb, p1 = p0 + p.ppb < HW ? p0 + p.ppb : HW;
-  const T* xs = x + n * xi.ns + (int64_t)q * V;
-  const T* ds = dy + n * di.ns + (int64_t)q * V;
-  T* os = dx + (int64_t)n * HW * C + (int64_t)q * V;
+  const T* xs = x + n * xi.ns + t.c0 + q * V;
+  const T* ds = dy + n * di.ns + t.c0 + q * V;
+  T* os = dx + (int64_t)n * HW * C + t.c0 + q * V;
   float mu[V], rs[V], ga[V], be[V], c1[V], c2[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const int c = q * V + e, g = n * G + c / (C / G);
-    mu[e] = mean[g];
-    rs[e] = rstd[g];
+    const int c = t.c0 + q * V + e, g = p.split == 1 ? (q * V + e) / p.D : 0, k = n * G + t.g0 + g;
+    mu[e] = mean[k];
+    rs[e] = rstd[k];
     ga[e] = gamma ? gamma[c] : 1.f;
     be[e] = beta ? beta[c] : 0.f;
-    c1[e] = coef[g];
-    c2[e] = coef[N * G + g];
+    c1[e] = stat[g].x;
+    c2[e] = stat[g].y;
   }
-  for (int64_t i = p0 + l; i < p1; i += p.pl) {
-    float r[V], d[V];
-    ldv<T, V>(xs + i * xi.ps, r);
-    ldv<T, V>(ds + i * di.ps, d);
+  walk<4>(p0 + l, p1, p.pl,
+          [&](int64_t i) {
+            return Two<T, V>{*reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps), *reinterpret_cast<const Vec<T, V>*>(ds + i * di.ps)};
+          },
+          [&](int64_t i, const Two<T, V>& r) {
+            float o[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float xh = (r[e] - mu[e]) * rs[e];
-      const float t = d[e] * act_bwd<ACT>(fmaf(xh, ga[e], be[e]), slope) * ga[e];
-      r[e] = rs[e] * (t - c1[e] - xh * c2[e]);
-    }
-    stv<T, V>(os + i * C, r);
-  }
+            for (int e = 0; e < V; ++e) {
+              const float xh = ((float)r.x.v[e] - mu[e]) * rs[e];
+              const float t1 = (float)r.d.v[e] * act_bwd<ACT>(fmaf(xh, ga[e], be[e]), slope) * ga[e];
+              o[e] = rs[e] * (t1 - c1[e] - xh * c2[e]);
+            }
+            stv<T, V>(os + i * C, o);
+          });
 }
 
 // ---------------------------------------------------------------- host side
 
-// widest vector that C, both strides and every pointer allow
-inline int vector_width(int esize, int C, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
+inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+constexpr int kMostVectors = 512;      // of a tile: its threads
+constexpr int64_t kMostThreads = (int64_t)1 << 32;   // of a launch
+constexpr int kFoldMost = 4096;        // partial results that a workgroup of the second pass folds by itself
+
+// widest vector that the channels, the strides and every pointer allow
+inline int vector_width(int esize, int C, int G, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
   for (int v = 16 / esize; v > 1; v /= 2) {
     bool ok = C % v == 0;
     for (const void* p : ptrs) ok = ok && (reinterpret_cast<uintptr_t>(p) % (v * esize)) == 0;
     for (int64_t s : strides) ok = ok && s % v == 0;
+    // a tile is whole groups that begin on the vector grid, or part of a group that does
+    const int D = C / G, u = v / gcd(D, v);
+    ok = ok && (C / v <= kMostVectors || (int64_t)u * D / v <= kMostVectors || D % v == 0);
     if (ok) return v;
   }
   return 1;
+}
+
+inline Plan make_plan(int N, int64_t HW, int C, int G, int V) {
+  Plan p;
+  p.D = C / G;
+  const int Q = C / V, u = V / gcd(p.D, V);
+  p.split = 1;
+  if (Q <= kMostVectors) {
+    p.gpt = G;
+    p.qt = Q;
+    p.tiles = 1;
+  } else if ((int64_t)u * p.D / V <= kMostVectors) {
+    const int run = u * p.D / V;
+    p.gpt = u * (kMostVectors / run);
+    p.qt = p.gpt * p.D / V;
+    p.tiles = (G + p.gpt - 1) / p.gpt;
+  } else {
+    const int w = p.D / V;
+    p.gpt = 1;
+    p.split = (w + kMostVectors - 1) / kMostVectors;
+    p.qt = (w + p.split - 1) / p.split;
+    p.split = (w + p.qt - 1) / p.qt;
+    p.tiles = G * p.split;
+  }
+  const int most = p.qt > 128 ? 512 : 256;
+  p.pl = most / p.qt > 1 ? most / p.qt : 1;
+  p.threads = (p.qt * p.pl + 63) / 64 * 64;
+  // about 1024 workgroups of 256 threads, with four pixels a thread or more
+  int64_t want = 262144 / p.threads / ((int64_t)N * p.tiles), can = (HW + p.pl * 4 - 1) / (p.pl * 4);
+  want = want < 1 ? 1 : want > 512 ? 512 : want;
+  p.nb = (int)(can < want ? can : want);
+  p.ppb = (HW + p.nb - 1) / p.nb;
+  p.nb = (int)((HW + p.ppb - 1) / p.ppb);                // no chunk is empty
+  return p;
+}
+
+// The small form: all values of a group fit the registers of one workgroup
+struct Small {
+  int dv, pl, threads;
+  bool ok;
+};
+template <int V>
+inline Small make_small(int N, int64_t HW, int C, int G, int esize) {
+  Small s;
+  const int D = C / G;
+  s.ok = false;
+  if (D % V || D / V > kSmallThreads<V>) return s;
+  s.dv = D / V;
+  s.pl = kSmallThreads<V> / s.dv;
+  if ((HW + s.pl - 1) / s.pl > kSmallVecs<V>) return s;
+  s.pl = (int)((HW + kSmallVecs<V> - 1) / kSmallVecs<V>);    // no more threads than the values need
+  s.threads = (s.dv * s.pl + 63) / 64 * 64;
+  s.ok = true;
+  return s;
 }
 
 template <class F>
@@ -379,17 +703,33 @@ int with_act(int act, F f) {
 template <class T>
 int forward(const T* x, Img xi, int N, int64_t HW, int C, int G, const float* gamma, const float* beta, float eps, int act, float slope, T* y,
             float* mean, float* rstd, float* ws, hipStream_t s) {
-  return with_vector(vector_width(sizeof(T), C, {x, y}, {xi.ns, xi.ps}), [&](auto vv) {
+  return with_vector(vector_width(sizeof(T), C, G, {x, y}, {xi.ns, xi.ps}), [&](auto vv) {
     constexpr int V = decltype(vv)::value;
     if constexpr (V * sizeof(T) <= 16) {
-      const Plan p = make_plan(N, HW, C, V);
-      const dim3 grid((unsigned)(p.tiles * p.nb * N));
-      hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(kThreads), p.pl * 2 * p.qt * V * sizeof(float), s, x, xi, p, N, HW, C, ws);
-      C3D_CHECK_LAUNCH();
-      hipLaunchKernelGGL(gn_fold_kernel, dim3(N * G), dim3(kThreads), 0, s, ws, p, N, HW, C, G, eps, mean, rstd);
-      C3D_CHECK_LAUNCH();
       return with_act(act, [&](auto aa) {
-        hipLaunchKernelGGL((gn_apply_kernel<T, V, decltype(aa)::value>), grid, dim3(kThreads), 0, s, x, xi, p, HW, C, G, mean, rstd, gamma, beta, slope, y);
+        constexpr int A = decltype(aa)::value;
+        const Small m = make_small<V>(N, HW, C, G, sizeof(T));
+        if (m.ok) {
+          C3D_REQUIRE((int64_t)N * G * m.threads < kMostThreads, "group_norm: too many samples and groups");
+          hipLaunchKernelGGL((gn_small_kernel<T, V, A>), dim3(N * G), dim3(m.threads), 0, s, x, xi, (int)HW, C, G, m.dv, m.pl, gamma, beta, eps, slope, y,
+                             mean, rstd);
+          C3D_CHECK_LAUNCH();
+          return 0;
+        }
+        const Plan p = make_plan(N, HW, C, G, V);
+        C3D_REQUIRE((int64_t)p.tiles * p.nb * N * p.threads < kMostThreads, "group_norm: too many samples and channels");
+        const dim3 grid((unsigned)(p.tiles * p.nb * N));
+        float2* part = reinterpret_cast<float2*>(ws);
+        const size_t lds = (size_t)(p.pl > 2 ? p.pl : 2) * p.qt * V * sizeof(float2);
+        hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(p.threads), lds, s, x, xi, p, HW, G, part);
+        C3D_CHECK_LAUNCH();
+        const bool fold = p.gpt * p.nb * p.split > kFoldMost;
+        if (fold) {
+          hipLaunchKernelGGL(gn_fold_kernel<V>, dim3((N * G + 3) / 4), dim3(64), 0, s, part, p, HW, N, G, eps, mean, rstd);
+          C3D_CHECK_LAUNCH();
+        }
+        hipLaunchKernelGGL((gn_apply_kernel<T, V, A>), grid, dim3(p.threads), p.gpt * sizeof(float2), s, x, xi, p, HW, C, G, fold ? nullptr : part, eps,
+                           mean, rstd, gamma, beta, slope, y);
         C3D_CHECK_LAUNCH();
         return 0;
       });
@@ -401,22 +741,45 @@ int forward(const T* x, Img xi, int N, int64_t HW, int C, int G, const float* ga
 template <class T>
 int backward(const T* dy, Img di, const T* x, Img xi, int N, int64_t HW, int C, int G, const float* mean, const float* rstd, const float* gamma,
              const float* beta, int act, float slope, T* dx, float* dgamma, float* dbeta, float* ws, hipStream_t s) {
-  return with_vector(vector_width(sizeof(T), C, {x, dy, dx}, {xi.ns, xi.ps, di.ns, di.ps}), [&](auto vv) {
+  return with_vector(vector_width(sizeof(T), C, G, {x, dy, dx}, {xi.ns, xi.ps, di.ns, di.ps}), [&](auto vv) {
     constexpr int V = decltype(vv)::value;
     if constexpr (V * sizeof(T) <= 16) {
-      const Plan p = make_plan(N, HW, C, V);
-      const dim3 grid((unsigned)(p.tiles * p.nb * N));
-      float* coef = ws + 2 * (int64_t)N * p.nb * C;
+      const bool wanted = dgamma || dbeta;
+      const int extra = wanted ? ((C + 15) / 16 + 7) / 8 * 8 : 0;      // of eights, so that a chunk keeps its XCD
       return with_act(act, [&](auto aa) {
         constexpr int A = decltype(aa)::value;
-        hipLaunchKernelGGL((gn_bwd_stats_kernel<T, V, A>), grid, dim3(kThreads), p.pl * 2 * p.qt * V * sizeof(float), s, dy, di, x, xi, p, N, HW, C, G,
-                           mean, rstd, gamma, beta, slope, ws);
+        const Small m = make_small<V>(N, HW, C, G, sizeof(T));
+        if (m.ok) {
+          float2* chan = reinterpret_cast<float2*>(ws);
+          const size_t lds = wanted ? (size_t)(m.pl + (m.pl > 1 ? (m.pl + 7) / 8 : 0)) * (C / G) * sizeof(float2) : 0;   // 49 KB at most
+          C3D_REQUIRE((int64_t)N * G * m.threads < kMostThreads, "group_norm_bwd: too many samples and groups");
+          hipLaunchKernelGGL((gn_small_bwd_kernel<T, V, A>), dim3(N * G), dim3(m.threads), lds, s, dy, di, x, xi, (int)HW, C, G, m.dv, m.pl, mean, rstd,
+                             gamma, beta, slope, dx, wanted ? chan : nullptr, dgamma, dbeta);
+          C3D_CHECK_LAUNCH();
+          if (wanted && N > 1) {
+            hipLaunchKernelGGL(gn_channels_kernel, dim3((C + 15) / 16), dim3(256), 0, s, chan, (int64_t)N, C, dgamma, dbeta);
+            C3D_CHECK_LAUNCH();
+          }
+          return 0;
+        }
+        const Plan p = make_plan(N, HW, C, G, V);
+        C3D_REQUIRE(((int64_t)p.tiles * p.nb * N + extra) * p.threads < kMostThreads, "group_norm_bwd: too many samples and channels");
+        const int blocks = p.tiles * p.nb * N;
+        float2* part = reinterpret_cast<float2*>(ws);
+        float2* chan = part + (int64_t)N * G * p.nb * p.split;
+        float2* coef = chan + (int64_t)N * p.nb * C;
+        const size_t lds = (size_t)(p.pl > 2 ? p.pl : 2) * p.qt * V * sizeof(float2);
+        hipLaunchKernelGGL((gn_bwd_stats_kernel<T, V, A>), dim3(blocks), dim3(p.threads), lds, s, dy, di, x, xi, p, HW, C, G, mean, rstd, gamma, beta,
+                           slope, part, wanted ? chan : nullptr);
         C3D_CHECK_LAUNCH();
-        hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3(N * G + (dgamma || dbeta ? C : 0)), dim3(kThreads), 0, s, ws, p, N, HW, C, G, gamma, coef, dgamma,
-                           dbeta);
-        C3D_CHECK_LAUNCH();
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, A>), grid, dim3(kThreads), 0, s, dy, di, x, xi, p, N, HW, C, G, mean, rstd, gamma, beta, slope, coef,
-                           dx);
+        const bool fold = p.gpt * p.nb * p.split > kFoldMost;
+        if (fold) {
+          hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3((N * G + 3) / 4), dim3(64), 0, s, part, p, HW, N, G, coef);
+          C3D_CHECK_LAUNCH();
+        }
+        const size_t lds2 = std::max(p.gpt * sizeof(float2), wanted ? 8 * 16 * sizeof(double2) : 0);
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, A>), dim3(blocks + extra), dim3(p.threads), lds2, s, dy, di, x, xi, p, HW, N, C, G, mean, rstd, gamma,
+                           beta, slope, fold ? coef : part, (int)fold, chan, extra, dgamma, dbeta, dx);
         C3D_CHECK_LAUNCH();
         return 0;
       });
@@ -431,7 +794,7 @@ int check(int N, int64_t HW, int C, int G, int type, int act, float slope) {
   C3D_REQUIRE(type >= 0 && type <= 2, "group_norm: type is 0 (fp32), 1 (bf16) or 2 (fp16)");
   C3D_REQUIRE(act >= ACT_NONE && act <= ACT_SILU, "group_norm: act is 0 (none), 1 (LeakyReLU) or 2 (SiLU)");
   C3D_REQUIRE(act != ACT_LRELU || (slope >= 0.f && slope <= 1.f), "group_norm: slope is in [0, 1]");
-  C3D_REQUIRE((int64_t)N * C < (int64_t)1 << 24 && C <= 1 << 20, "group_norm: too many samples or channels");
+  C3D_REQUIRE((int64_t)N * C < (int64_t)1 << 31 && C <= 1 << 20, "group_norm: too many samples or channels");
   return 0;
 }
 
@@ -439,13 +802,16 @@ int check(int N, int64_t HW, int C, int G, int type, int act, float slope) {
 
 extern "C" int64_t c3d_group_norm_ws_floats(int N, int64_t HW, int C, int G, int type) {
   if (check(N, HW, C, G, type, 0, 0.f) || N == 0 || HW == 0) return 0;
-  int64_t most = 0;
+  int64_t most = 2 * (int64_t)N * C;                     // the small form's rows
   for (int v = 16 / (type == 0 ? 4 : 2); v >= 1; v /= 2) {
     if (C % v) continue;
-    const int64_t f = 2 * (int64_t)N * make_plan(N, HW, C, v).nb * C;
+    const int D = C / G, u = v / gcd(D, v);
+    if (!(C / v <= kMostVectors || (int64_t)u * D / v <= kMostVectors || D % v == 0)) continue;
+    const Plan p = make_plan(N, HW, C, G, v);
+    const int64_t f = 2 * ((int64_t)N * G * p.nb * p.split + (int64_t)N * p.nb * C + (int64_t)N * G);
     most = f > most ? f : most;
   }
-  return most + 2 * (int64_t)N * G;
+  return most;
 }
 
 extern "C" int c3d_group_norm(const void* x, int64_t x_ns, int64_t x_ps, int N, int64_t HW, int C, int G, int type, const float* gamma,

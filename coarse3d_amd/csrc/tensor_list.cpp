@@ -36,8 +36,26 @@ bool same_layout(const at::Tensor& a, const at::Tensor& b) {
   return true;
 }
 
+// The common case, in one pass: every list ascends in memory and no two lists interleave (`ends`: where each list's ranges end)
+bool plainly_disjoint(const std::vector<Range>& r, const std::vector<size_t>& ends) {
+  std::vector<Range> hull;
+  size_t i = 0;
+  for (size_t end : ends) {
+    if (i == end) continue;
+    for (size_t k = i + 1; k < end; ++k)
+      if (r[k].lo < r[k - 1].hi) return false;
+    hull.push_back({r[i].lo, r[end - 1].hi, true});
+    i = end;
+  }
+  for (size_t a = 0; a < hull.size(); ++a)
+    for (size_t b = a + 1; b < hull.size(); ++b)
+      if (hull[a].lo < hull[b].hi && hull[b].lo < hull[a].hi) return false;
+  return true;
+}
+
 // two ranges of which one is written share memory
-bool overlapping(std::vector<Range>& r) {
+bool overlapping(std::vector<Range>& r, const std::vector<size_t>& ends) {
+  if (plainly_disjoint(r, ends)) return false;
   auto before = [](const Range& a, const Range& b) { return a.lo < b.lo; };
   if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
   uintptr_t any = 0, written = 0;      // ends of what came before
@@ -85,6 +103,7 @@ PyObject* pack_impl(PyObject* args) {
   c3d_opt_tensor* rec = reinterpret_cast<c3d_opt_tensor*>(PyBytes_AS_STRING(out));
   std::vector<Range> ranges;
   ranges.reserve((size_t)count * kSlots);
+  std::vector<size_t> ends;
   at::ScalarType type[kSlots];
   c10::Device device(c10::kCPU);
   bool seen = false;
@@ -146,8 +165,9 @@ PyObject* pack_impl(PyObject* args) {
         ranges.push_back({lo, lo + (uintptr_t)n * t.element_size(), kinds[s] != 'r'});
       }
     }
+    ends.push_back(ranges.size());
   }
-  if (bad.empty() && overlapping(ranges)) bad = what + "two tensors share memory";
+  if (bad.empty() && overlapping(ranges, ends)) bad = what + "two tensors share memory";
   if (bad.empty() && count > 0 && !device.is_cuda()) bad = what + "the tensors are on " + device.str() + ", not on a GPU";
   if (!bad.empty()) {
     Py_DECREF(out);

@@ -851,7 +851,7 @@ def _grad_norm(records, max_norm, what):
         raise ValueError(f"{what}: max_norm is not negative, got {max_norm}")
     buf, n, index, ty = records
     dev = torch.device("cuda", index)
-    part = torch.empty(L.lib().c3d_grad_norm_partials(buf, n), device=dev, dtype=torch.float64)
+    part = torch.empty(L.lib().c3d_grad_norm_partials(buf, n, ty), device=dev, dtype=torch.float64)
     out = torch.empty(2, device=dev, dtype=torch.float32)
     norm, scale = out[0], out[1]
     _call_on(index, "c3d_grad_norm", buf, n, ty, max_norm, _dp(part), _dp(norm), _dp(scale))

@@ -330,7 +330,7 @@ int c3d_sums_to_f32(const double* sums, int C, int col, float* out, int accumula
  * dx alike); gamma, beta [C] fp32 (NULL: 1, 0).  act: 0 none, 1 LeakyReLU(slope), 2 SiLU.
  *   mean, rstd [N][G] : of the HW * C / G values of (n, g), biased variance, rstd = 1 / sqrt(var + eps)
  *   y = act((x - mean) * rstd * gamma + beta)
- * ws: c3d_group_norm_ws_floats() floats.  N * HW == 0 is allowed (nothing to normalise).                            */
+ * ws: c3d_group_norm_ws_floats() floats, 8-byte aligned.  N * HW == 0 is allowed (nothing to normalise).                            */
 int64_t c3d_group_norm_ws_floats(int N, int64_t HW, int C, int G, int type);
 int c3d_group_norm(const void* x, int64_t x_ns, int64_t x_ps, int N, int64_t HW, int C, int G, int type,
                    const float* gamma, const float* beta, float eps, int act, float slope, void* y, float* mean,
@@ -355,7 +355,7 @@ typedef struct {
 /* elements that share one scale of an 8-bit state                                                                 */
 #define C3D_ADAMW8_BLOCK 256
 /* number of doubles of c3d_grad_norm's workspace (host call)                                                       */
-int64_t c3d_grad_norm_partials(const c3d_opt_tensor* t, int count);
+int64_t c3d_grad_norm_partials(const c3d_opt_tensor* t, int count, int type);
 /* *norm = sqrt(sum of all squares) (sums in 64 bits, fixed order), *scale = min(1, max_norm / (norm + 1e-6)): the factor of
  * torch.nn.utils.clip_grad_norm_, for c3d_scale_tensors or c3d_adamw_desc.grad_scale.  type as above.               */
 int c3d_grad_norm(const c3d_opt_tensor* t, int count, int type, double max_norm, double* partial, float* norm,

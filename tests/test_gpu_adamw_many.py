@@ -1,5 +1,5 @@
-"""ops.grad_norm / clip_grad_norm_ / adamw_step / adamw8_step against float64, and the 8-bit states against a bit-exact float32 restatement
-in numpy (numpy rounds every float32 operation once, to nearest: what the kernel is written to do for everything that decides a code).
+"""ops.grad_norm / clip_grad_norm_ / adamw_step / adamw8_step against float64, and the 8-bit states bit for bit against a restatement of their
+rule in numpy: scales from float32 operations that are each rounded once (as the kernel's are), codes from float64.
 
 Tolerances: u = 2^-24.  m is two products and a sum (3 roundings), v three products and a sum (4), the new parameter carries one rounding of
 the decay product, one of the sum, and the update's own: m 3 u, the root u (half of v's 4, plus its own) and eps' sum, the division (at most
@@ -108,9 +108,9 @@ def np_bits(blocks_before, n, step, seed):
 E4M3 = np.array([float(x) for x in torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).float()], np.float32)
 
 
-def np_encode(x, rnd16, floor):
-    """float32 values -> (codes, scales), element by element from the rule: the grid point below |x| / scale, or the one above where
-    the fraction plus rnd16 / 2^16 reaches one; in the subnormal range the fraction is first rounded to 2^-20."""
+def np_encode(x, wide, rnd16, floor):
+    """x: the float32 values, which decide the scale; wide: the same in float64, which decide the codes: the grid point below
+    |wide| / scale, or the one above where the fraction plus rnd16 / 2^16 reaches one."""
     n = x.size
     codes, scales = np.zeros(n, np.uint8), np.zeros((n + 255) // 256, np.float32)
     grid = E4M3[:127].astype(np.float64)
@@ -119,22 +119,14 @@ def np_encode(x, rnd16, floor):
         xs, r = x[s], rnd16[s].astype(np.float64)
         fin = np.isfinite(xs)
         top = float(np.max(np.abs(xs[fin]), initial=0.0))
-        k = max(-100, math.ceil(math.log2(top / 448.0)) if top > 0 else -1000)
-        if top > 0:                                     # exact whatever log2 rounded
-            while k > -100 and top <= 448.0 * 2.0 ** (k - 1):
-                k -= 1
-            while top > 448.0 * 2.0 ** k:
-                k += 1
+        k = -100
+        while top > 448.0 * 2.0 ** k:
+            k += 1
         scales[b] = 2.0 ** k
-        a = np.abs(np.where(fin, xs, 0)).astype(np.float64) / 2.0 ** k
-        a = a.astype(np.float32).astype(np.float64)
-        low = a < 2.0 ** -6
-        a = np.where(low, np.round(a * 2.0 ** 29) / 2.0 ** 29, a)      # np.round: ties to even, as the sum does
+        a = np.minimum(np.abs(np.where(fin, wide[s], 0)) / 2.0 ** k, 448.0)
         i = np.searchsorted(grid, a, side="right") - 1
-        nxt = grid[np.minimum(i + 1, 126)]
-        width = np.where(i < 126, nxt - grid[i], 32.0)
-        up = (a - grid[i]) / width + r / 65536.0 >= 1.0
-        c = np.minimum(i + up, 126)
+        width = np.where(i < 126, grid[np.minimum(i + 1, 126)] - grid[i], 32.0)
+        c = np.minimum(i + ((a - grid[i]) / width + r / 65536.0 >= 1.0), 126)
         if floor:
             c = np.where((xs > 0) & (c == 0), 1, c)
         c = np.where(fin, c, 127).astype(np.uint8)
@@ -151,8 +143,11 @@ def np_step8(g, m8, ms, r8, rs, before, step, seed, b1=0.9, b2=0.999, scale=np.f
         m = E4M3[m8] * rep(ms) * f(b1) + x * f(1 - b1)
         old = E4M3[r8] * rep(rs)
         r = np.sqrt((old * old) * f(b2) + (x * x) * f(1 - b2))
+        d = np.float64
+        wide_m = (E4M3[m8] * rep(ms)).astype(d) * b1 + x.astype(d) * (1 - b1)
+        wide_r = np.sqrt(old.astype(d) ** 2 * b2 + x.astype(d) ** 2 * (1 - b2))
     bits = np_bits(before, n, step, seed)
-    return m, r, np_encode(m, bits & 0xFFFF, False), np_encode(r, bits >> np.uint32(16), True)
+    return m, r, np_encode(m, wide_m, bits & 0xFFFF, False), np_encode(r, wide_r, bits >> np.uint32(16), True)
 
 
 def state8(sizes):
