@@ -30,11 +30,17 @@ __device__ __forceinline__ void ldv(const T* p, float (&r)[V]) {
 #pragma unroll
   for (int q = 0; q < V; ++q) r[q] = (float)t.v[q];
 }
-template <class T, int V>
+// NT: past the caches
+template <class T, int V, bool NT = false>
 __device__ __forceinline__ void stv(T* p, const float (&r)[V]) {
   Vec<T, V> t;
 #pragma unroll
   for (int q = 0; q < V; ++q) t.v[q] = (T)r[q];
+  if constexpr (NT && sizeof(t) == 16) {
+    typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, t), reinterpret_cast<u32x4_t*>(p));
+    return;
+  }
   *reinterpret_cast<Vec<T, V>*>(p) = t;
 }
 
@@ -66,11 +72,18 @@ template <int V>
 constexpr int kSmallVecs = V == 8 ? 4 : 16 / V;        // vectors a thread holds
 // thread t: vector t % dv of the group's D / V, pixels t / dv + r * pl
 
+// sum over the workgroup, the same bits in every thread; red: 16 floats that the last sum did not use
 __device__ __forceinline__ float block_sum(float v, float* red) {
-  v = c3d_wave_sum(v);
-  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[w] = v;
+#define C3D_SUM_STEP(ctrl, rows) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, rows, 0xf, false))
+  C3D_SUM_STEP(0x111, 0xf);      // row_shr:1, 2, 4, 8: lane 15 of a row of sixteen has the row's
+  C3D_SUM_STEP(0x112, 0xf);
+  C3D_SUM_STEP(0x114, 0xf);
+  C3D_SUM_STEP(0x118, 0xf);
+  C3D_SUM_STEP(0x142, 0xa);      // row_bcast:15 into rows 1 and 3, row_bcast:31 into 2 and 3: lane 63 has all
+  C3D_SUM_STEP(0x143, 0xc);
+#undef C3D_SUM_STEP
+  const int nw = blockDim.x >> 6;
+  if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
   __syncthreads();
   float s = 0.f;
   for (int i = 0; i < nw; ++i) s += red[i];
@@ -83,13 +96,19 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_kernel(const T* __r
                                                                   float slope, T* __restrict__ y, float* __restrict__ mean,
                                                                   float* __restrict__ rstd) {
   constexpr int R = kSmallVecs<V>;
-  __shared__ float red[16];
+  __shared__ float red[32];
   const int n = blockIdx.x / G, g = blockIdx.x % G, l = threadIdx.x / dv, c = g * (C / G) + (threadIdx.x % dv) * V;
   const T* xs = x + n * xi.ns + c;
   Vec<T, V> raw[R];
 #pragma unroll
   for (int r = 0; r < R; ++r)
     if (l < pl && l + r * pl < HW) raw[r] = *reinterpret_cast<const Vec<T, V>*>(xs + (int64_t)(l + r * pl) * xi.ps);
+  float ga[V], be[V];                                    // (c is a channel of the group for idle threads too)
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    ga[e] = gamma ? gamma[c + e] : 1.f;
+    be[e] = beta ? beta[c + e] : 0.f;
+  }
   const float count = (float)HW * (float)(C / G);
   float s = 0.f;
 #pragma unroll
@@ -107,18 +126,12 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_kernel(const T* __r
         const float d = (float)raw[r].v[e] - mu;
         s = fmaf(d, d, s);
       }
-  const float rs = 1.f / sqrtf(block_sum(s, red) / count + eps);
+  const float rs = 1.f / sqrtf(block_sum(s, red + 16) / count + eps);
   if (threadIdx.x == 0) {
     mean[blockIdx.x] = mu;
     rstd[blockIdx.x] = rs;
   }
   if (l >= pl) return;
-  float ga[V], be[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    ga[e] = gamma ? gamma[c + e] : 1.f;
-    be[e] = beta ? beta[c + e] : 0.f;
-  }
   T* ys = y + (int64_t)n * HW * C + c;
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -135,12 +148,12 @@ template <class T, int V, int ACT>
 __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_bwd_kernel(const T* __restrict__ dy, Img di, const T* __restrict__ x, Img xi, int HW, int C,
                                                                       int G, int dv, int pl, const float* __restrict__ mean,
                                                                       const float* __restrict__ rstd, const float* __restrict__ gamma,
-                                                                      const float* __restrict__ beta, float slope, T* __restrict__ dx,
+                                                                      const float* __restrict__ beta, float slope, T* __restrict__ dx, int wanted,
                                                                       float2* __restrict__ chan, float* __restrict__ dgamma,
                                                                       float* __restrict__ dbeta) {
   constexpr int R = kSmallVecs<V>;
   extern __shared__ float2 rows[];                       // [pl][D], then [pl / 8][D]
-  __shared__ float red[16];
+  __shared__ float red[32];
   const int n = blockIdx.x / G, g = blockIdx.x % G, D = C / G, l = threadIdx.x / dv, q = threadIdx.x % dv, c = g * D + q * V;
   const T* xs = x + n * xi.ns + c;
   const T* ds = dy + n * di.ns + c;
@@ -176,7 +189,7 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_bwd_kernel(const T*
     s2 = fmaf(b[e], ga[e], s2);
   }
   const float count = (float)HW * (float)D;
-  const float c1 = block_sum(s1, red) / count, c2 = block_sum(s2, red) / count;
+  const float c1 = block_sum(s1, red) / count, c2 = block_sum(s2, red + 16) / count;
   if (l < pl) {
     T* os = dx + (int64_t)n * HW * C + c;
 #pragma unroll
@@ -192,7 +205,7 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_bwd_kernel(const T*
         stv<T, V>(os + (int64_t)(l + r * pl) * C, o);
       }
   }
-  if (!chan) return;
+  if (!wanted) return;
   // the channels' sums: eight rows to one until one is left
   if (l < pl)
 #pragma unroll
@@ -228,11 +241,19 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_bwd_kernel(const T*
 // ---------------------------------------------------------------- large: two passes
 
 // How an image is cut.  A tile of channels is `gpt` whole groups (split == 1), or one of `split` parts of a group too wide for a
-// workgroup; qt vectors wide, `pl` pixels side by side.  A sample's pixels are cut into nb chunks of ppb.
+// workgroup; qt vectors wide, `pl` pixels side by side.  A sample's pixels are cut into runs of kRun * pl, and of nb workgroups the
+// b-th takes runs b, b + nb, ...: at any time the workgroups read one window of memory together, and the second pass, which begins
+// with the last runs, finds the latest of it in the caches (8x64x2048x32 fp32, both passes: 82 us; with a chunk of its own each 86).
+constexpr int kRun = 8;
 struct Plan {
   int D, qt, pl, threads, tiles, gpt, split, nb;
-  int64_t ppb;
+  int64_t runs;
 };
+// pixels of workgroup b
+__host__ __device__ inline int64_t pixels_of(const Plan& p, int64_t HW, int b) {
+  const int64_t mine = (p.runs - b + p.nb - 1) / p.nb, run = (int64_t)kRun * p.pl;
+  return mine * run - ((p.runs - 1) % p.nb == b ? p.runs * run - HW : 0);
+}
 struct Tile {
   int c0, nq, g0, ng, part;      // first channel, vectors, first group, groups, part of the group
 };
@@ -260,29 +281,47 @@ __device__ __forceinline__ int backwards(int b, int n) {
   return b < whole ? whole - 8 - (b & ~7) + (b & 7) : b;
 }
 
-// sums of a pair over the 16 lanes of a DPP row, in 64 bits
-__device__ __forceinline__ void sum16(double& a, double& b) {
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
+// sums of a pair over `lanes` (a power of two) neighbouring lanes, in 64 bits
+__device__ __forceinline__ void sum_lanes(double& a, double& b, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
     a += __shfl_xor(a, o, 64);
     b += __shfl_xor(b, o, 64);
   }
+}
+// Lanes that work on a group together, such that all of a tile's groups are worked on at once where the workgroup has the threads;
+// `body(group, lane)` is called by whole waves, with groups past the last too
+template <class F>
+__device__ __forceinline__ void for_groups(int ng, F body) {
+  int lanes = 64;
+  while (lanes > 16 && ng * lanes > (int)blockDim.x) lanes >>= 1;
+  const int per = 64 / lanes;
+  for (int g = threadIdx.x / lanes; g < (ng + per - 1) / per * per; g += blockDim.x / lanes) body(g, (int)(threadIdx.x & (lanes - 1)), lanes);
 }
 
 // Partial results: [N][G][nb][split] pairs, part_at() the first of a chunk
 __device__ __forceinline__ int64_t part_at(const Plan& p, int G, int n, int g) { return ((int64_t)n * G + g) * p.nb * p.split; }
 
-// unrolled walk over a chunk's pixels: U loads in flight ahead of their use
-template <int U, class F, class H>
-__device__ __forceinline__ void walk(int64_t i, int64_t end, int step, F load, H use) {
-  for (; i + (int64_t)(U - 1) * step < end; i += (int64_t)U * step) {
-    decltype(load(i)) r[U];
+// a thread's pixels of its workgroup's runs, U loads in flight ahead of their use; BACK: from the last run to the first
+template <int U, bool BACK, class F, class H>
+__device__ __forceinline__ void walk(const Plan& p, int64_t HW, int b, int l, F load, H use) {
+  static_assert(kRun % U == 0, "a run is taken in whole steps");
+  const int64_t last = b + (p.runs - 1 - b) / p.nb * p.nb, run = (int64_t)kRun * p.pl;
+  for (int64_t k = b; k <= last; k += p.nb) {
+    const int64_t at = BACK ? last + b - k : k;
+    int64_t i = at * run + l;
+    if ((at + 1) * run <= HW) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) r[u] = load(i + (int64_t)u * step);
+      for (int h = 0; h < kRun; h += U, i += (int64_t)U * p.pl) {
+        decltype(load(i)) r[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) use(i + (int64_t)u * step, r[u]);
+        for (int u = 0; u < U; ++u) r[u] = load(i + (int64_t)u * p.pl);
+#pragma unroll
+        for (int u = 0; u < U; ++u) use(i + (int64_t)u * p.pl, r[u]);
+      }
+    } else {
+      for (; i < HW; i += p.pl) use(i, load(i));
+    }
   }
-  for (; i < end; i += step) use(i, load(i));
 }
 
 // sums of s1, s2 [V] over the workgroup's `pl` pixel lanes: -> shared sum[ch] of the tile's channels
@@ -308,8 +347,8 @@ __device__ __forceinline__ void join_lanes(const Plan& p, const Tile& t, bool on
   __syncthreads();
 }
 
-// First pass: mean and sum of squared deviations of every group in the chunk.  Values are shifted by the chunk's first pixel, so that
-// a mean far from zero costs nothing.
+// First pass: mean and sum of squared deviations of every group over the workgroup's pixels.  Values are shifted by its first pixel, so that a mean
+// far from zero costs nothing.
 template <class T, int V>
 __global__ __launch_bounds__(512) void gn_stats_kernel(const T* __restrict__ x, Img xi, Plan p, int64_t HW, int G, float2* __restrict__ part) {
   extern __shared__ float2 sum[];
@@ -317,14 +356,13 @@ __global__ __launch_bounds__(512) void gn_stats_kernel(const T* __restrict__ x, 
   const int b = (blockIdx.x / p.tiles) % p.nb, n = blockIdx.x / (p.tiles * p.nb);
   const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
   const bool on = l < p.pl && q < t.nq;
-  const int64_t p0 = b * p.ppb, p1 = p0 + p.ppb < HW ? p0 + p.ppb : HW;
   float shift[V], s1[V], s2[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) shift[e] = s1[e] = s2[e] = 0.f;
   if (on) {
     const T* xs = x + n * xi.ns + t.c0 + q * V;
-    ldv<T, V>(xs + p0 * xi.ps, shift);
-    walk<8>(p0 + l, p1, p.pl, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); },
+    ldv<T, V>(xs + (int64_t)b * kRun * p.pl * xi.ps, shift);
+    walk<8, false>(p, HW, b, l, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); },
             [&](int64_t, const Vec<T, V>& r) {
 #pragma unroll
               for (int e = 0; e < V; ++e) {
@@ -335,62 +373,61 @@ __global__ __launch_bounds__(512) void gn_stats_kernel(const T* __restrict__ x, 
             });
   }
   join_lanes<V>(p, t, on, l, q, s1, s2, sum);
-  const float cnt = (float)(p1 - p0);
+  const double cnt = (double)pixels_of(p, HW, b);
   float2* shifts = sum + p.qt * V;                        // (row 1: free again)
   if (on && l == 0)
 #pragma unroll
     for (int e = 0; e < V; ++e) shifts[q * V + e].x = shift[e];
   __syncthreads();
-  // sixteen lanes a group: mean and deviations over its channels
   const int chans = p.split == 1 ? p.D : t.nq * V;
-  for (int g = threadIdx.x / 16; g < (t.ng + 3) / 4 * 4; g += blockDim.x / 16) {
+  for_groups(t.ng, [&](int g, int lane, int lanes) {
     double m = 0.0, m2 = 0.0;
     if (g < t.ng)
-      for (int k = threadIdx.x % 16; k < chans; k += 16) {
+      for (int k = lane; k < chans; k += lanes) {
         const float2 v = sum[g * p.D + k];
         const double d = (double)v.x / cnt, mu = (double)shifts[g * p.D + k].x + d;
         m += mu;
         m2 += ((double)v.y - (double)v.x * d) + cnt * mu * mu;
       }
-    sum16(m, m2);
-    if (g < t.ng && threadIdx.x % 16 == 0) {
+    sum_lanes(m, m2, lanes);
+    if (g < t.ng && lane == 0) {
       const double mu = m / chans;
       part[part_at(p, G, n, t.g0 + g) + b * p.split + t.part] = make_float2((float)mu, (float)fmax(m2 - cnt * chans * mu * mu, 0.0));
     }
-  }
+  });
 }
 
-// mean and rstd of (n, g) from its partial results, by sixteen lanes; every lane gets them
-__device__ __forceinline__ float2 fold_stats(const float2* __restrict__ part, const Plan& p, int V, int64_t HW, int G, int n, int g, float eps) {
+// mean and rstd of (n, g) from its partial results, by `lanes` lanes; every lane gets them
+__device__ __forceinline__ float2 fold_stats(const float2* __restrict__ part, const Plan& p, int V, int64_t HW, int G, int n, int g, float eps, int lane,
+                                             int lanes) {
   const float2* a = part + part_at(p, G, n, g);
   double s = 0.0, s2 = 0.0;
-  for (int i = threadIdx.x % 16; i < p.nb * p.split; i += 16) {
-    const int b = i / p.split, k = i % p.split;
-    const int64_t p0 = b * p.ppb, p1 = p0 + p.ppb < HW ? p0 + p.ppb : HW;
-    const double cnt = (double)(p1 - p0) * (p.split == 1 ? p.D : min(p.qt * V, p.D - k * p.qt * V));
+#pragma unroll 4
+  for (int i = lane; i < p.nb * p.split; i += lanes) {
+    const int b = p.split == 1 ? i : i / p.split, k = i - b * p.split;
+    const double cnt = (double)pixels_of(p, HW, b) * (p.split == 1 ? p.D : min(p.qt * V, p.D - k * p.qt * V));
     const float2 v = a[i];
     s += cnt * v.x;
     s2 += (double)v.y + cnt * ((double)v.x * v.x);
   }
-  sum16(s, s2);
+  sum_lanes(s, s2, lanes);
   const double M = (double)HW * p.D, mu = s / M, var = s2 / M - mu * mu;
   return make_float2((float)mu, (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)eps)));
 }
 
+// a wave each, for tiles of many groups
 template <int V>
-__global__ __launch_bounds__(64) void gn_fold_kernel(const float2* __restrict__ part, Plan p, int64_t HW, int N, int G, float eps, float* __restrict__ mean,
+__global__ __launch_bounds__(64) void gn_fold_kernel(const float2* __restrict__ part, Plan p, int64_t HW, int G, float eps, float* __restrict__ mean,
                                                     float* __restrict__ rstd) {
-  const int i = blockIdx.x * 4 + threadIdx.x / 16;
-  const int k = min(i, N * G - 1);
-  const float2 r = fold_stats(part, p, V, HW, G, k / G, k % G, eps);
-  if (i < N * G && threadIdx.x % 16 == 0) {
-    mean[i] = r.x;
-    rstd[i] = r.y;
+  const float2 r = fold_stats(part, p, V, HW, G, blockIdx.x / G, blockIdx.x % G, eps, threadIdx.x, 64);
+  if (threadIdx.x == 0) {
+    mean[blockIdx.x] = r.x;
+    rstd[blockIdx.x] = r.y;
   }
 }
 
 // Second pass.  part != NULL: the statistics are still in pieces; every workgroup folds those of its groups
-template <class T, int V, int ACT>
+template <class T, int V, int ACT, bool NT>
 __global__ __launch_bounds__(512) void gn_apply_kernel(const T* __restrict__ x, Img xi, Plan p, int64_t HW, int C, int G, const float2* __restrict__ part,
                                                       float eps, float* __restrict__ mean, float* __restrict__ rstd,
                                                       const float* __restrict__ gamma, const float* __restrict__ beta, float slope,
@@ -399,21 +436,20 @@ __global__ __launch_bounds__(512) void gn_apply_kernel(const T* __restrict__ x, 
   const int block = backwards(blockIdx.x, gridDim.x);
   const Tile t = tile_of<V>(p, block % p.tiles, G);
   const int b = (block / p.tiles) % p.nb, n = block / (p.tiles * p.nb);
-  for (int g = threadIdx.x / 16; g < (t.ng + 3) / 4 * 4; g += blockDim.x / 16) {
+  for_groups(t.ng, [&](int g, int lane, int lanes) {
     const int k = n * G + t.g0 + min(g, t.ng - 1);
-    const float2 r = part ? fold_stats(part, p, V, HW, G, n, k - n * G, eps) : make_float2(mean[k], rstd[k]);
-    if (g < t.ng && threadIdx.x % 16 == 0) {
+    const float2 r = part ? fold_stats(part, p, V, HW, G, n, k - n * G, eps, lane, lanes) : make_float2(mean[k], rstd[k]);
+    if (g < t.ng && lane == 0) {
       stat[g] = r;
       if (part && b == 0 && t.part == 0) {
         mean[k] = r.x;
         rstd[k] = r.y;
       }
     }
-  }
+  });
   __syncthreads();
   const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
   if (l >= p.pl || q >= t.nq) return;
-  const int64_t p0 = b * p.ppb, p1 = p0 + p.ppb < HW ? p0 + p.ppb : HW;
   const T* xs = x + n * xi.ns + t.c0 + q * V;
   T* ys = y + (int64_t)n * HW * C + t.c0 + q * V;
   float mu[V], rs[V], ga[V], be[V];
@@ -426,12 +462,12 @@ __global__ __launch_bounds__(512) void gn_apply_kernel(const T* __restrict__ x, 
     ga[e] = gamma ? gamma[c] : 1.f;
     be[e] = beta ? beta[c] : 0.f;
   }
-  walk<4>(p0 + l, p1, p.pl, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); },
+  walk<8, true>(p, HW, b, l, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); },
           [&](int64_t i, const Vec<T, V>& r) {
             float o[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) o[e] = act_fwd<ACT>(fmaf(((float)r.v[e] - mu[e]) * rs[e], ga[e], be[e]), slope);
-            stv<T, V>(ys + i * C, o);
+            stv<T, V, NT>(ys + i * C, o);
           });
 }
 
@@ -451,7 +487,6 @@ __global__ __launch_bounds__(512) void gn_bwd_stats_kernel(const T* __restrict__
   const int b = (blockIdx.x / p.tiles) % p.nb, n = blockIdx.x / (p.tiles * p.nb);
   const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
   const bool on = l < p.pl && q < t.nq;
-  const int64_t p0 = b * p.ppb, p1 = p0 + p.ppb < HW ? p0 + p.ppb : HW;
   float s1[V], s2[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
@@ -467,7 +502,7 @@ __global__ __launch_bounds__(512) void gn_bwd_stats_kernel(const T* __restrict__
       ga[e] = gamma ? gamma[c] : 1.f;
       be[e] = beta ? beta[c] : 0.f;
     }
-    walk<4>(p0 + l, p1, p.pl,
+    walk<8, false>(p, HW, b, l,
             [&](int64_t i) {
               return Two<T, V>{*reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps), *reinterpret_cast<const Vec<T, V>*>(ds + i * di.ps)};
             },
@@ -485,37 +520,36 @@ __global__ __launch_bounds__(512) void gn_bwd_stats_kernel(const T* __restrict__
   if (chan)
     for (int i = threadIdx.x; i < t.nq * V; i += blockDim.x) chan[((int64_t)n * p.nb + b) * C + t.c0 + i] = sum[i];
   const int chans = p.split == 1 ? p.D : t.nq * V;
-  for (int g = threadIdx.x / 16; g < (t.ng + 3) / 4 * 4; g += blockDim.x / 16) {
+  for_groups(t.ng, [&](int g, int lane, int lanes) {
     double a = 0.0, c = 0.0;
     if (g < t.ng)
-      for (int k = threadIdx.x % 16; k < chans; k += 16) {
+      for (int k = lane; k < chans; k += lanes) {
         const float2 v = sum[g * p.D + k];
         const double ga = gamma ? (double)gamma[t.c0 + g * p.D + k] : 1.0;
         a += ga * v.x;
         c += ga * v.y;
       }
-    sum16(a, c);
-    if (g < t.ng && threadIdx.x % 16 == 0) part[part_at(p, G, n, t.g0 + g) + b * p.split + t.part] = make_float2((float)a, (float)c);
-  }
+    sum_lanes(a, c, lanes);
+    if (g < t.ng && lane == 0) part[part_at(p, G, n, t.g0 + g) + b * p.split + t.part] = make_float2((float)a, (float)c);
+  });
 }
 
-// the means of t and t xhat over (n, g), by sixteen lanes
-__device__ __forceinline__ float2 fold_means(const float2* __restrict__ part, const Plan& p, int64_t HW, int G, int n, int g) {
+// the means of t and t xhat over (n, g), by `lanes` lanes
+__device__ __forceinline__ float2 fold_means(const float2* __restrict__ part, const Plan& p, int64_t HW, int G, int n, int g, int lane, int lanes) {
   const float2* a = part + part_at(p, G, n, g);
   double s = 0.0, s2 = 0.0;
-  for (int i = threadIdx.x % 16; i < p.nb * p.split; i += 16) {
+#pragma unroll 4
+  for (int i = lane; i < p.nb * p.split; i += lanes) {
     s += (double)a[i].x;
     s2 += (double)a[i].y;
   }
-  sum16(s, s2);
+  sum_lanes(s, s2, lanes);
   const double M = (double)HW * p.D;
   return make_float2((float)(s / M), (float)(s2 / M));
 }
-__global__ __launch_bounds__(64) void gn_bwd_fold_kernel(const float2* __restrict__ part, Plan p, int64_t HW, int N, int G, float2* __restrict__ coef) {
-  const int i = blockIdx.x * 4 + threadIdx.x / 16;
-  const int k = min(i, N * G - 1);
-  const float2 r = fold_means(part, p, HW, G, k / G, k % G);
-  if (i < N * G && threadIdx.x % 16 == 0) coef[i] = r;
+__global__ __launch_bounds__(64) void gn_bwd_fold_kernel(const float2* __restrict__ part, Plan p, int64_t HW, int G, float2* __restrict__ coef) {
+  const float2 r = fold_means(part, p, HW, G, blockIdx.x / G, blockIdx.x % G, threadIdx.x, 64);
+  if (threadIdx.x == 0) coef[blockIdx.x] = r;
 }
 
 // dgamma, dbeta of 16 channels: the rows of chan [rows][C], in 64 bits and a fixed order
@@ -553,7 +587,7 @@ __global__ __launch_bounds__(256) void gn_channels_kernel(const float2* __restri
 }
 
 // Backward, second pass.  The first `extra` workgroups fold dgamma and dbeta; folded: part holds [N][G] means already
-template <class T, int V, int ACT>
+template <class T, int V, int ACT, bool NT>
 __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(const T* __restrict__ dy, Img di, const T* __restrict__ x, Img xi, Plan p, int64_t HW, int N,
                                                           int C, int G, const float* __restrict__ mean, const float* __restrict__ rstd,
                                                           const float* __restrict__ gamma, const float* __restrict__ beta, float slope,
@@ -567,15 +601,14 @@ __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(const T* __restrict__
   const int block = backwards(blockIdx.x - extra, gridDim.x - extra);
   const Tile t = tile_of<V>(p, block % p.tiles, G);
   const int b = (block / p.tiles) % p.nb, n = block / (p.tiles * p.nb);
-  for (int g = threadIdx.x / 16; g < (t.ng + 3) / 4 * 4; g += blockDim.x / 16) {
+  for_groups(t.ng, [&](int g, int lane, int lanes) {
     const int k = t.g0 + min(g, t.ng - 1);
-    const float2 r = folded ? part[n * G + k] : fold_means(part, p, HW, G, n, k);
-    if (g < t.ng && threadIdx.x % 16 == 0) stat[g] = r;
-  }
+    const float2 r = folded ? part[n * G + k] : fold_means(part, p, HW, G, n, k, lane, lanes);
+    if (g < t.ng && lane == 0) stat[g] = r;
+  });
   __syncthreads();
   const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
   if (l >= p.pl || q >= t.nq) return;
-  const int64_t p0 = b * p.ppb, p1 = p0 + p.ppb < HW ? p0 + p.ppb : HW;
   const T* xs = x + n * xi.ns + t.c0 + q * V;
   const T* ds = dy + n * di.ns + t.c0 + q * V;
   T* os = dx + (int64_t)n * HW * C + t.c0 + q * V;
@@ -590,7 +623,7 @@ __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(const T* __restrict__
     c1[e] = stat[g].x;
     c2[e] = stat[g].y;
   }
-  walk<4>(p0 + l, p1, p.pl,
+  walk<4, true>(p, HW, b, l,
           [&](int64_t i) {
             return Two<T, V>{*reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps), *reinterpret_cast<const Vec<T, V>*>(ds + i * di.ps)};
           },
@@ -602,7 +635,7 @@ __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(const T* __restrict__
               const float t1 = (float)r.d.v[e] * act_bwd<ACT>(fmaf(xh, ga[e], be[e]), slope) * ga[e];
               o[e] = rs[e] * (t1 - c1[e] - xh * c2[e]);
             }
-            stv<T, V>(os + i * C, o);
+            stv<T, V, NT>(os + i * C, o);
           });
 }
 
@@ -615,14 +648,14 @@ constexpr int64_t kMostThreads = (int64_t)1 << 32;   // of a launch
 constexpr int kFoldMost = 4096;        // partial results that a workgroup of the second pass folds by itself
 
 // widest vector that the channels, the strides and every pointer allow
-inline int vector_width(int esize, int C, int G, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
+inline int vector_width(int esize, int C, int G, bool small, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
   for (int v = 16 / esize; v > 1; v /= 2) {
     bool ok = C % v == 0;
     for (const void* p : ptrs) ok = ok && (reinterpret_cast<uintptr_t>(p) % (v * esize)) == 0;
     for (int64_t s : strides) ok = ok && s % v == 0;
-    // a tile is whole groups that begin on the vector grid, or part of a group that does
+    // small: a group is whole vectors.  Large: a tile is whole groups that begin on the vector grid, or part of a group that does
     const int D = C / G, u = v / gcd(D, v);
-    ok = ok && (C / v <= kMostVectors || (int64_t)u * D / v <= kMostVectors || D % v == 0);
+    ok = ok && (small ? D % v == 0 : C / v <= kMostVectors || (int64_t)u * D / v <= kMostVectors || D % v == 0);
     if (ok) return v;
   }
   return 1;
@@ -653,34 +686,32 @@ inline Plan make_plan(int N, int64_t HW, int C, int G, int V) {
   const int most = p.qt > 128 ? 512 : 256;
   p.pl = most / p.qt > 1 ? most / p.qt : 1;
   p.threads = (p.qt * p.pl + 63) / 64 * 64;
-  // about 1024 workgroups of 256 threads, with four pixels a thread or more
-  int64_t want = 262144 / p.threads / ((int64_t)N * p.tiles), can = (HW + p.pl * 4 - 1) / (p.pl * 4);
+  // about 1024 workgroups of 256 threads
+  p.runs = (HW + (int64_t)kRun * p.pl - 1) / ((int64_t)kRun * p.pl);
+  int64_t want = 262144 / p.threads / ((int64_t)N * p.tiles);
   want = want < 1 ? 1 : want > 512 ? 512 : want;
-  p.nb = (int)(can < want ? can : want);
-  p.ppb = (HW + p.nb - 1) / p.nb;
-  p.nb = (int)((HW + p.ppb - 1) / p.ppb);                // no chunk is empty
+  p.nb = (int)(p.runs < want ? p.runs : want);
   return p;
 }
 
-// The small form: all values of a group fit the registers of one workgroup
+// The small form takes what fits the registers of one workgroup whatever the vector width: 16 values a thread of 1024 (512 with 32)
+inline bool is_small(int64_t HW, int D) { return D <= 1024 && HW <= 16 * (1024 / D); }
 struct Small {
   int dv, pl, threads;
-  bool ok;
 };
 template <int V>
-inline Small make_small(int N, int64_t HW, int C, int G, int esize) {
+inline Small make_small(int64_t HW, int D) {
   Small s;
-  const int D = C / G;
-  s.ok = false;
-  if (D % V || D / V > kSmallThreads<V>) return s;
   s.dv = D / V;
-  s.pl = kSmallThreads<V> / s.dv;
-  if ((HW + s.pl - 1) / s.pl > kSmallVecs<V>) return s;
-  s.pl = (int)((HW + kSmallVecs<V> - 1) / kSmallVecs<V>);    // no more threads than the values need
+  const int64_t most = kSmallThreads<V> / s.dv;
+  s.pl = (int)(HW < most ? HW : most);
   s.threads = (s.dv * s.pl + 63) / 64 * 64;
-  s.ok = true;
   return s;
 }
+
+// A result larger than the eight L2 caches goes past them and the infinity cache: its reader would not find it there, and what it does
+// not push out is the input that this pass still has to read (8x64x2048x32 fp32: 80 -> 67 us, its step in bf16 with 704 channels 164 -> 148)
+inline bool past_caches(int N, int64_t HW, int C, int esize) { return (int64_t)N * HW * C * esize > (32 << 20); }
 
 template <class F>
 int with_vector(int v, F f) {
@@ -703,13 +734,14 @@ int with_act(int act, F f) {
 template <class T>
 int forward(const T* x, Img xi, int N, int64_t HW, int C, int G, const float* gamma, const float* beta, float eps, int act, float slope, T* y,
             float* mean, float* rstd, float* ws, hipStream_t s) {
-  return with_vector(vector_width(sizeof(T), C, G, {x, y}, {xi.ns, xi.ps}), [&](auto vv) {
+  const bool small = is_small(HW, C / G);
+  return with_vector(vector_width(sizeof(T), C, G, small, {x, y}, {xi.ns, xi.ps}), [&](auto vv) {
     constexpr int V = decltype(vv)::value;
     if constexpr (V * sizeof(T) <= 16) {
       return with_act(act, [&](auto aa) {
         constexpr int A = decltype(aa)::value;
-        const Small m = make_small<V>(N, HW, C, G, sizeof(T));
-        if (m.ok) {
+        if (small) {
+          const Small m = make_small<V>(HW, C / G);
           C3D_REQUIRE((int64_t)N * G * m.threads < kMostThreads, "group_norm: too many samples and groups");
           hipLaunchKernelGGL((gn_small_kernel<T, V, A>), dim3(N * G), dim3(m.threads), 0, s, x, xi, (int)HW, C, G, m.dv, m.pl, gamma, beta, eps, slope, y,
                              mean, rstd);
@@ -725,10 +757,12 @@ int forward(const T* x, Img xi, int N, int64_t HW, int C, int G, const float* ga
         C3D_CHECK_LAUNCH();
         const bool fold = p.gpt * p.nb * p.split > kFoldMost;
         if (fold) {
-          hipLaunchKernelGGL(gn_fold_kernel<V>, dim3((N * G + 3) / 4), dim3(64), 0, s, part, p, HW, N, G, eps, mean, rstd);
+          hipLaunchKernelGGL(gn_fold_kernel<V>, dim3(N * G), dim3(64), 0, s, part, p, HW, G, eps, mean, rstd);
           C3D_CHECK_LAUNCH();
         }
-        hipLaunchKernelGGL((gn_apply_kernel<T, V, A>), grid, dim3(p.threads), p.gpt * sizeof(float2), s, x, xi, p, HW, C, G, fold ? nullptr : part, eps,
+        // (only whole vectors of 16 bytes have the form that goes past the caches)
+        const auto apply = V * sizeof(T) == 16 && past_caches(N, HW, C, sizeof(T)) ? gn_apply_kernel<T, V, A, V * sizeof(T) == 16> : gn_apply_kernel<T, V, A, false>;
+        hipLaunchKernelGGL(apply, grid, dim3(p.threads), p.gpt * sizeof(float2), s, x, xi, p, HW, C, G, fold ? nullptr : part, eps,
                            mean, rstd, gamma, beta, slope, y);
         C3D_CHECK_LAUNCH();
         return 0;
@@ -741,20 +775,21 @@ int forward(const T* x, Img xi, int N, int64_t HW, int C, int G, const float* ga
 template <class T>
 int backward(const T* dy, Img di, const T* x, Img xi, int N, int64_t HW, int C, int G, const float* mean, const float* rstd, const float* gamma,
              const float* beta, int act, float slope, T* dx, float* dgamma, float* dbeta, float* ws, hipStream_t s) {
-  return with_vector(vector_width(sizeof(T), C, G, {x, dy, dx}, {xi.ns, xi.ps, di.ns, di.ps}), [&](auto vv) {
+  const bool small = is_small(HW, C / G);
+  return with_vector(vector_width(sizeof(T), C, G, small, {x, dy, dx}, {xi.ns, xi.ps, di.ns, di.ps}), [&](auto vv) {
     constexpr int V = decltype(vv)::value;
     if constexpr (V * sizeof(T) <= 16) {
       const bool wanted = dgamma || dbeta;
       const int extra = wanted ? ((C + 15) / 16 + 7) / 8 * 8 : 0;      // of eights, so that a chunk keeps its XCD
       return with_act(act, [&](auto aa) {
         constexpr int A = decltype(aa)::value;
-        const Small m = make_small<V>(N, HW, C, G, sizeof(T));
-        if (m.ok) {
+        if (small) {
+          const Small m = make_small<V>(HW, C / G);
           float2* chan = reinterpret_cast<float2*>(ws);
           const size_t lds = wanted ? (size_t)(m.pl + (m.pl > 1 ? (m.pl + 7) / 8 : 0)) * (C / G) * sizeof(float2) : 0;   // 49 KB at most
           C3D_REQUIRE((int64_t)N * G * m.threads < kMostThreads, "group_norm_bwd: too many samples and groups");
           hipLaunchKernelGGL((gn_small_bwd_kernel<T, V, A>), dim3(N * G), dim3(m.threads), lds, s, dy, di, x, xi, (int)HW, C, G, m.dv, m.pl, mean, rstd,
-                             gamma, beta, slope, dx, wanted ? chan : nullptr, dgamma, dbeta);
+                             gamma, beta, slope, dx, (int)wanted, chan, dgamma, dbeta);
           C3D_CHECK_LAUNCH();
           if (wanted && N > 1) {
             hipLaunchKernelGGL(gn_channels_kernel, dim3((C + 15) / 16), dim3(256), 0, s, chan, (int64_t)N, C, dgamma, dbeta);
@@ -774,11 +809,13 @@ int backward(const T* dy, Img di, const T* x, Img xi, int N, int64_t HW, int C, 
         C3D_CHECK_LAUNCH();
         const bool fold = p.gpt * p.nb * p.split > kFoldMost;
         if (fold) {
-          hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3((N * G + 3) / 4), dim3(64), 0, s, part, p, HW, N, G, coef);
+          hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3(N * G), dim3(64), 0, s, part, p, HW, G, coef);
           C3D_CHECK_LAUNCH();
         }
         const size_t lds2 = std::max(p.gpt * sizeof(float2), wanted ? 8 * 16 * sizeof(double2) : 0);
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, A>), dim3(blocks + extra), dim3(p.threads), lds2, s, dy, di, x, xi, p, HW, N, C, G, mean, rstd, gamma,
+        const auto apply =
+            V * sizeof(T) == 16 && past_caches(N, HW, C, sizeof(T)) ? gn_bwd_apply_kernel<T, V, A, V * sizeof(T) == 16> : gn_bwd_apply_kernel<T, V, A, false>;
+        hipLaunchKernelGGL(apply, dim3(blocks + extra), dim3(p.threads), lds2, s, dy, di, x, xi, p, HW, N, C, G, mean, rstd, gamma,
                            beta, slope, fold ? coef : part, (int)fold, chan, extra, dgamma, dbeta, dx);
         C3D_CHECK_LAUNCH();
         return 0;
@@ -802,7 +839,8 @@ int check(int N, int64_t HW, int C, int G, int type, int act, float slope) {
 
 extern "C" int64_t c3d_group_norm_ws_floats(int N, int64_t HW, int C, int G, int type) {
   if (check(N, HW, C, G, type, 0, 0.f) || N == 0 || HW == 0) return 0;
-  int64_t most = 2 * (int64_t)N * C;                     // the small form's rows
+  if (is_small(HW, C / G)) return N > 1 ? 2 * (int64_t)N * C : 0;
+  int64_t most = 0;
   for (int v = 16 / (type == 0 ? 4 : 2); v >= 1; v /= 2) {
     if (C % v) continue;
     const int D = C / G, u = v / gcd(D, v);
@@ -819,7 +857,7 @@ extern "C" int c3d_group_norm(const void* x, int64_t x_ns, int64_t x_ps, int N, 
   if (int rc = check(N, HW, C, G, type, act, slope)) return rc;
   C3D_REQUIRE(eps >= 0.f, "group_norm: eps is negative or not a number");
   if (N == 0 || HW == 0) return 0;
-  C3D_REQUIRE(x && y && mean && rstd && ws, "group_norm: null pointer");
+  C3D_REQUIRE(x && y && mean && rstd && (ws || is_small(HW, C / G)), "group_norm: null pointer");
   C3D_REQUIRE(x_ps >= C && (N == 1 || x_ns >= (HW - 1) * x_ps + C), "group_norm: strides overlap");
   const Img xi{x_ns, x_ps};
   hipStream_t s = (hipStream_t)stream;
@@ -833,7 +871,7 @@ extern "C" int c3d_group_norm_bwd(const void* dy, int64_t dy_ns, int64_t dy_ps, 
                                   void* dx, float* dgamma, float* dbeta, float* ws, c3d_stream stream) {
   if (int rc = check(N, HW, C, G, type, act, slope)) return rc;
   if (N == 0 || HW == 0) return 0;
-  C3D_REQUIRE(x && dy && dx && mean && rstd && ws, "group_norm_bwd: null pointer");
+  C3D_REQUIRE(x && dy && dx && mean && rstd && (ws || (N == 1 && is_small(HW, C / G))), "group_norm_bwd: null pointer");
   C3D_REQUIRE(x_ps >= C && (N == 1 || x_ns >= (HW - 1) * x_ps + C), "group_norm_bwd: strides of x overlap");
   C3D_REQUIRE(dy_ps >= C && (N == 1 || dy_ns >= (HW - 1) * dy_ps + C), "group_norm_bwd: strides of dy overlap");
   const Img xi{x_ns, x_ps}, di{dy_ns, dy_ps};
