@@ -71,20 +71,23 @@ class AdamWDesc(C.Structure):
 
 
 _lib = None
-_tlist = None
+_nat = None
 
 
-def tensor_list():
-    """The native module that turns lists of tensors into the records of the many-tensor entry points (csrc/tensor_list.cpp)."""
-    global _tlist
-    if _tlist is None:
+def native():
+    """The CPython module over torch's C++ API that does the host side of short calls (csrc/native.cpp)."""
+    global _nat
+    if _nat is None:
         try:
-            from . import _tensor_list
+            from . import _native
         except ImportError as e:
-            raise RuntimeError("coarse3d_amd/_tensor_list.so is missing or does not load: the extension has not been built (run "
+            raise RuntimeError("coarse3d_amd/_native.so is missing or does not load: the extension has not been built (run "
                                "`python -c 'import __graft_entry__ as g; g.build()'`). There is no fallback.") from e
-        _tlist = _tensor_list
-    return _tlist
+        address = lambda f: C.cast(f, C.c_void_p).value  # noqa: E731
+        k = lib()
+        _native.bind(address(k.c3d_group_norm), address(k.c3d_group_norm_bwd), address(k.c3d_group_norm_ws_floats), address(k.c3d_last_error))
+        _nat = _native
+    return _nat
 
 
 def lib():

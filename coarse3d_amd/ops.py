@@ -728,53 +728,15 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 # ---------------------------------------------------------------------------- GroupNorm with an activation
-_ACTS = {"none": 0, "lrelu": 1, "silu": 2}
-
-
-def _pixel_rows(t, what):
-    """(samples, pixels, channels, elements from sample to sample, from pixel to pixel) of a channels-last tensor [N, ..., C]."""
-    if t.dim() < 2:
-        raise ValueError(f"{what} is [N, ..., C], got {tuple(t.shape)}")
-    n, c = t.shape[0], t.shape[-1]
-    if t.numel() == 0:
-        return n, (0 if c and n else 1), c, 0, c
-    if t.is_contiguous():
-        hw = t.numel() // (n * c)
-        return n, hw, c, hw * c, c
-    st, hw, ps = t.stride(), 1, None
-    ok = c == 1 or st[-1] == 1
-    for d in range(t.dim() - 2, 0, -1):
-        if t.shape[d] > 1:
-            if ps is None:
-                ps = st[d]
-            ok = ok and st[d] == ps * hw
-            hw *= t.shape[d]
-    ps = c if ps is None else ps
-    ns = st[0] if n > 1 else hw * ps
-    if not ok or ps < c or (n > 1 and ns < (hw - 1) * ps + c):
-        raise ValueError(f"{what}: the channels of a pixel have to lie side by side and the pixels one stride apart; got shape "
-                         f"{tuple(t.shape)}, strides {st} (call .contiguous())")
-    return n, hw, c, ns, ps
-
-
-def _affine_vectors(gamma, beta, c, device):
-    for t, name in ((gamma, "gamma"), (beta, "beta")):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (c,) or not t.is_contiguous() or t.device != device):
-            raise ValueError(f"group_norm: {name} is a contiguous fp32 tensor of {c} values on {device}")
-
-
-def _gn_check(x, act, slope, what):
-    if x.dtype not in _TYPES:
-        raise ValueError(f"{what}: fp32, bf16 or fp16, got {x.dtype}")
-    if act not in _ACTS:
-        raise ValueError(f"{what}: act is one of {sorted(_ACTS)}, got {act!r}")
-    if not 0.0 <= slope <= 1.0:
-        raise ValueError(f"{what}: slope is in [0, 1], got {slope}")
-
-
-def _on_gpu(t, what):
-    if not t.is_cuda:
-        raise ValueError(f"{what}: the tensors are on {t.device}, not on a GPU")
+def _on_device_of(x, call, *args):
+    """call(*args, stream) with x's device current; a tensor elsewhere than on a GPU is left for the call to refuse."""
+    index = x.get_device()
+    if index < 0:
+        return call(*args, 0)
+    if index == _cur_dev():
+        return call(*args, _stream().value or 0)
+    with torch.cuda.device(index):
+        return call(*args, _stream().value or 0)
 
 
 def group_norm(x, groups, gamma=None, beta=None, eps=1e-5, act="lrelu", slope=0.01):
@@ -783,53 +745,13 @@ def group_norm(x, groups, gamma=None, beta=None, eps=1e-5, act="lrelu", slope=0.
     or None.  act: "none", "lrelu" (``slope``; 0 = ReLU) or "silu".  Returns (y, mean, rstd): y dense and of x's type, mean / rstd
     [N, groups] fp32 for ``group_norm_bwd``.  Sums are fp32 or wider, y is rounded once.  A sample that holds a value which is not
     finite gives NaN in that value's group and nowhere else."""
-    _gn_check(x, act, slope, "group_norm")
-    n, hw, c, ns, ps = _pixel_rows(x, "group_norm: x")
-    if groups < 1 or c < 1 or c % groups:
-        raise ValueError(f"group_norm: {c} channels do not divide into {groups} groups")
-    if not eps >= 0.0:
-        raise ValueError(f"group_norm: eps is not negative, got {eps}")
-    _affine_vectors(gamma, beta, c, x.device)
-    _on_gpu(x, "group_norm")
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    if n == 0 or hw == 0:
-        return y, torch.zeros(n, groups, device=x.device), torch.zeros(n, groups, device=x.device)
-    ty = _TYPES[x.dtype]
-    stats = torch.empty(2, n, groups, device=x.device, dtype=torch.float32)
-    mean, rstd = stats[0], stats[1]
-    ws = torch.empty(L.lib().c3d_group_norm_ws_floats(n, hw, c, groups, ty), device=x.device, dtype=torch.float32)
-    _call_on(x.get_device(), "c3d_group_norm", _dp(x), ns, ps, n, hw, c, groups, ty, _dp(gamma), _dp(beta), eps, _ACTS[act], slope, _dp(y), _dp(mean),
-             _dp(rstd), _dp(ws))
-    return y, mean, rstd
+    return _on_device_of(x, L.native().group_norm, x, groups, gamma, beta, eps, act, slope)
 
 
 def group_norm_bwd(dy, x, mean, rstd, gamma=None, beta=None, act="lrelu", slope=0.01):
     """Gradients of ``group_norm``: (dx, dgamma, dbeta), dx dense and of x's type, dgamma / dbeta [C] fp32 (None where the
     parameter is None).  Deterministic: partial sums are folded in a fixed order."""
-    _gn_check(x, act, slope, "group_norm_bwd")
-    n, hw, c, ns, ps = _pixel_rows(x, "group_norm_bwd: x")
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
-        raise ValueError(f"group_norm_bwd: dy is {tuple(dy.shape)} {dy.dtype} on {dy.device}, x is {tuple(x.shape)} {x.dtype} on {x.device}")
-    _, _, _, dns, dps = _pixel_rows(dy, "group_norm_bwd: dy")
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t.dim() != 2 or t.shape[0] != n or t.shape != mean.shape or t.dtype != torch.float32 or not t.is_contiguous() or t.device != x.device:
-            raise ValueError(f"group_norm_bwd: {name} is the fp32 [N, groups] tensor that group_norm returned")
-    groups = mean.shape[1]
-    if groups < 1 or c < 1 or c % groups:
-        raise ValueError(f"group_norm_bwd: {c} channels do not divide into {groups} groups")
-    _affine_vectors(gamma, beta, c, x.device)
-    _on_gpu(x, "group_norm_bwd")
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    if n == 0 or hw == 0:
-        z = torch.zeros(2, c, device=x.device)
-        return dx, z[0] if gamma is not None else None, z[1] if beta is not None else None
-    ty = _TYPES[x.dtype]
-    dgamma = torch.empty(c, device=x.device, dtype=torch.float32) if gamma is not None else None
-    dbeta = torch.empty(c, device=x.device, dtype=torch.float32) if beta is not None else None
-    ws = torch.empty(L.lib().c3d_group_norm_ws_floats(n, hw, c, groups, ty), device=x.device, dtype=torch.float32)
-    _call_on(x.get_device(), "c3d_group_norm_bwd", _dp(dy), dns, dps, _dp(x), ns, ps, n, hw, c, groups, ty, _dp(mean), _dp(rstd), _dp(gamma), _dp(beta),
-             _ACTS[act], slope, _dp(dx), _dp(dgamma), _dp(dbeta), _dp(ws))
-    return dx, dgamma, dbeta
+    return _on_device_of(x, L.native().group_norm_bwd, dy, x, mean, rstd, gamma, beta, act, slope)
 
 
 # ---------------------------------------------------------------------------- optimiser over many tensors
@@ -838,7 +760,7 @@ _GRAD_NAMES = ("", "grads", "", "", "", "", "")
 
 
 def _grad_records(grads, kind, what):
-    buf, n, index, types = L.tensor_list().pack(what, (None, grads, None, None, None, None, None), "w" + kind + "wwwww", _GRAD_NAMES)
+    buf, n, index, types = L.native().pack(what, (None, grads, None, None, None, None, None), "w" + kind + "wwwww", _GRAD_NAMES)
     if n == 0:
         raise ValueError(f"{what}: no tensors")
     if types[1] not in _TYPES:
@@ -882,7 +804,7 @@ def _device_scalar(t, index, what):
 
 
 def _adamw(what, lists, kinds, names, bits, step, lr, betas, eps, weight_decay, grad_scale, seed):
-    buf, n, index, types = L.tensor_list().pack(what, lists, kinds, names)
+    buf, n, index, types = L.native().pack(what, lists, kinds, names)
     if n == 0:
         raise ValueError(f"{what}: no tensors")
     p, g, m, v, ms, vs, w = types

@@ -34,7 +34,7 @@ def test_group_norm_refusals(kw, match):
 
 @pytest.mark.parametrize("kw,match", [
     (dict(dy=torch.ones(2, 3, 4)), "dy"), (dict(dy=torch.ones(2, 3, 8).half()), "dy"), (dict(mean=torch.ones(2, 3)), "rstd"), (dict(mean=torch.ones(3, 2)), "mean"),
-    (dict(rstd=torch.ones(2, 2).double()), "rstd"), (dict(mean=torch.ones(2, 3), rstd=torch.ones(2, 3)), "divide"), (dict(act=1), "act"), (dict(), "on cpu"),
+    (dict(rstd=torch.ones(2, 2).double()), "rstd"), (dict(mean=torch.ones(2, 3), rstd=torch.ones(2, 3)), "divide"), (dict(act="relu6"), "act"), (dict(), "on cpu"),
 ])
 def test_group_norm_bwd_refusals(kw, match):
     kw = dict(dict(dy=torch.ones(2, 3, 8), x=torch.ones(2, 3, 8), mean=torch.ones(2, 2), rstd=torch.ones(2, 2)), **kw)
@@ -118,6 +118,6 @@ def test_the_library_refuses_what_the_wrappers_would_not_send():
     assert lib.c3d_grad_norm(rec, 1, 0, 1.0, None, 8, 8, None) == 2 and lib.c3d_scale_tensors(rec, 1, 0, None, None) == 2
     gn = lambda **k: lib.c3d_group_norm(*dict(dict(x=16, ns=24, ps=8, N=2, HW=3, C=8, G=2, type=0, ga=None, be=None, eps=1e-5, act=1, slope=0.01, y=16,  # noqa: E731
                                                    mean=16, rstd=16, ws=16, s=None), **k).values())
-    for k in (dict(G=3), dict(N=-1), dict(HW=-1), dict(type=5), dict(act=9), dict(slope=2.0), dict(eps=-1.0), dict(x=None), dict(ws=None), dict(ps=7), dict(ns=23)):
+    for k in (dict(G=3), dict(N=-1), dict(HW=-1), dict(type=5), dict(act=9), dict(slope=2.0), dict(eps=-1.0), dict(x=None), dict(ws=None, HW=100000, ns=800000), dict(ps=7), dict(ns=23)):
         assert gn(**k) == 2, k
     assert gn(N=0) == 0 and gn(HW=0) == 0
