@@ -44,17 +44,20 @@ __device__ __forceinline__ void stv(T* p, const float (&r)[V]) {
   *reinterpret_cast<Vec<T, V>*>(p) = t;
 }
 
+// 1 / (1 + e^-z) from the hardware's exp2 and reciprocal: off by a few units in the last place, and by |z| of them for z far below
+// zero, where the result itself vanishes
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
 template <int ACT>
 __device__ __forceinline__ float act_fwd(float z, float slope) {
   if (ACT == ACT_LRELU) return z > 0.f ? z : z * slope;
-  if (ACT == ACT_SILU) return z / (1.f + expf(-z));
+  if (ACT == ACT_SILU) return z * sigmoid(z);
   return z;
 }
 template <int ACT>
 __device__ __forceinline__ float act_bwd(float z, float slope) {
   if (ACT == ACT_LRELU) return z > 0.f ? 1.f : slope;
   if (ACT == ACT_SILU) {
-    const float s = 1.f / (1.f + expf(-z));
+    const float s = sigmoid(z);
     return s * (1.f + z * (1.f - s));
   }
   return 1.f;
@@ -244,16 +247,15 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_bwd_kernel(const T*
 // workgroup; qt vectors wide, `pl` pixels side by side.  A sample's pixels are cut into runs of kRun * pl, and of nb workgroups the
 // b-th takes runs b, b + nb, ...: at any time the workgroups read one window of memory together, and the second pass, which begins
 // with the last runs, finds the latest of it in the caches (8x64x2048x32 fp32, both passes: 82 us; with a chunk of its own each 86).
-constexpr int kRun = 8;
+constexpr int kRun = 4;
 struct Plan {
   int D, qt, pl, threads, tiles, gpt, split, nb;
-  int64_t runs;
+  int64_t each;             // every workgroup takes this many runs, and the first `more` one more
+  int more;
+  int run, last, missing;   // pixels of a run; the workgroup that has the last one, and how many pixels that one lacks
 };
-// pixels of workgroup b
-__host__ __device__ inline int64_t pixels_of(const Plan& p, int64_t HW, int b) {
-  const int64_t mine = (p.runs - b + p.nb - 1) / p.nb, run = (int64_t)kRun * p.pl;
-  return mine * run - ((p.runs - 1) % p.nb == b ? p.runs * run - HW : 0);
-}
+__device__ __forceinline__ int64_t runs_of(const Plan& p, int b) { return p.each + (b < p.more ? 1 : 0); }
+__device__ __forceinline__ int64_t pixels_of(const Plan& p, int b) { return runs_of(p, b) * p.run - (b == p.last ? p.missing : 0); }
 struct Tile {
   int c0, nq, g0, ng, part;      // first channel, vectors, first group, groups, part of the group
 };
@@ -301,27 +303,50 @@ __device__ __forceinline__ void for_groups(int ng, F body) {
 // Partial results: [N][G][nb][split] pairs, part_at() the first of a chunk
 __device__ __forceinline__ int64_t part_at(const Plan& p, int G, int n, int g) { return ((int64_t)n * G + g) * p.nb * p.split; }
 
-// a thread's pixels of its workgroup's runs, U loads in flight ahead of their use; BACK: from the last run to the first
-template <int U, bool BACK, class F, class H>
-__device__ __forceinline__ void walk(const Plan& p, int64_t HW, int b, int l, F load, H use) {
-  static_assert(kRun % U == 0, "a run is taken in whole steps");
-  const int64_t last = b + (p.runs - 1 - b) / p.nb * p.nb, run = (int64_t)kRun * p.pl;
-  for (int64_t k = b; k <= last; k += p.nb) {
-    const int64_t at = BACK ? last + b - k : k;
-    int64_t i = at * run + l;
-    if ((at + 1) * run <= HW) {
+// A thread's pixels of its workgroup's runs, all loads of a run in flight together; BACK: from the last run to the first.  (Fetching the
+// next run ahead as well costs the registers of a wave and loses 1-7 %.)
+template <bool BACK, class F>
+struct Walk {
+  using R = std::invoke_result_t<F, int64_t>;
+  const Plan& p;
+  int64_t HW;
+  int b, l;
+  F load;
+  R ahead[kRun];
+  // first pixel of the k-th run in the walk's order
+  __device__ __forceinline__ int64_t at(int64_t k) const { return ((BACK ? runs_of(p, b) - 1 - k : k) * p.nb + b) * p.run + l; }
+  __device__ __forceinline__ void fetch(int64_t i) {
+    if (i + (kRun - 1) * p.pl < HW) {
 #pragma unroll
-      for (int h = 0; h < kRun; h += U, i += (int64_t)U * p.pl) {
-        decltype(load(i)) r[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) r[u] = load(i + (int64_t)u * p.pl);
-#pragma unroll
-        for (int u = 0; u < U; ++u) use(i + (int64_t)u * p.pl, r[u]);
-      }
+      for (int u = 0; u < kRun; ++u) ahead[u] = load(i + u * p.pl);
     } else {
-      for (; i < HW; i += p.pl) use(i, load(i));
+#pragma unroll
+      for (int u = 0; u < kRun; ++u)
+        if (i + u * p.pl < HW) ahead[u] = load(i + u * p.pl);
     }
   }
+  // issues the first run's loads: what else has to be waited for ahead of `each` is waited for together with them
+  __device__ __forceinline__ void begin() { fetch(at(0)); }
+  template <class H>
+  __device__ __forceinline__ void each(H use) {
+    const int64_t runs = runs_of(p, b);
+    for (int64_t k = 0; k < runs; ++k) {
+      const int64_t i = at(k);
+      if (k) fetch(i);
+      if (i + (kRun - 1) * p.pl < HW) {
+#pragma unroll
+        for (int u = 0; u < kRun; ++u) use(i + u * p.pl, ahead[u]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kRun; ++u)
+          if (i + u * p.pl < HW) use(i + u * p.pl, ahead[u]);
+      }
+    }
+  }
+};
+template <bool BACK, class F>
+__device__ __forceinline__ Walk<BACK, F> walk(const Plan& p, int64_t HW, int b, int l, F load) {
+  return Walk<BACK, F>{p, HW, b, l, load};
 }
 
 // sums of s1, s2 [V] over the workgroup's `pl` pixel lanes: -> shared sum[ch] of the tile's channels
@@ -361,9 +386,10 @@ __global__ __launch_bounds__(512) void gn_stats_kernel(const T* __restrict__ x, 
   for (int e = 0; e < V; ++e) shift[e] = s1[e] = s2[e] = 0.f;
   if (on) {
     const T* xs = x + n * xi.ns + t.c0 + q * V;
-    ldv<T, V>(xs + (int64_t)b * kRun * p.pl * xi.ps, shift);
-    walk<8, false>(p, HW, b, l, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); },
-            [&](int64_t, const Vec<T, V>& r) {
+    auto w = walk<false>(p, HW, b, l, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); });
+    w.begin();
+    ldv<T, V>(xs + (int64_t)b * p.run * xi.ps, shift);
+    w.each([&](int64_t, const Vec<T, V>& r) {
 #pragma unroll
               for (int e = 0; e < V; ++e) {
                 const float d = (float)r.v[e] - shift[e];
@@ -373,7 +399,7 @@ __global__ __launch_bounds__(512) void gn_stats_kernel(const T* __restrict__ x, 
             });
   }
   join_lanes<V>(p, t, on, l, q, s1, s2, sum);
-  const double cnt = (double)pixels_of(p, HW, b);
+  const double cnt = (double)pixels_of(p, b);
   float2* shifts = sum + p.qt * V;                        // (row 1: free again)
   if (on && l == 0)
 #pragma unroll
@@ -405,7 +431,7 @@ __device__ __forceinline__ float2 fold_stats(const float2* __restrict__ part, co
 #pragma unroll 4
   for (int i = lane; i < p.nb * p.split; i += lanes) {
     const int b = p.split == 1 ? i : i / p.split, k = i - b * p.split;
-    const double cnt = (double)pixels_of(p, HW, b) * (p.split == 1 ? p.D : min(p.qt * V, p.D - k * p.qt * V));
+    const double cnt = (double)pixels_of(p, b) * (p.split == 1 ? p.D : min(p.qt * V, p.D - k * p.qt * V));
     const float2 v = a[i];
     s += cnt * v.x;
     s2 += (double)v.y + cnt * ((double)v.x * v.x);
@@ -436,6 +462,12 @@ __global__ __launch_bounds__(512) void gn_apply_kernel(const T* __restrict__ x, 
   const int block = backwards(blockIdx.x, gridDim.x);
   const Tile t = tile_of<V>(p, block % p.tiles, G);
   const int b = (block / p.tiles) % p.nb, n = block / (p.tiles * p.nb);
+  const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
+  const bool on = l < p.pl && q < t.nq;
+  const T* xs = x + n * xi.ns + t.c0 + q * V;
+  T* ys = y + (int64_t)n * HW * C + t.c0 + q * V;
+  auto w = walk<true>(p, HW, b, l, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); });
+  if (on) w.begin();
   for_groups(t.ng, [&](int g, int lane, int lanes) {
     const int k = n * G + t.g0 + min(g, t.ng - 1);
     const float2 r = part ? fold_stats(part, p, V, HW, G, n, k - n * G, eps, lane, lanes) : make_float2(mean[k], rstd[k]);
@@ -448,10 +480,7 @@ __global__ __launch_bounds__(512) void gn_apply_kernel(const T* __restrict__ x, 
     }
   });
   __syncthreads();
-  const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
-  if (l >= p.pl || q >= t.nq) return;
-  const T* xs = x + n * xi.ns + t.c0 + q * V;
-  T* ys = y + (int64_t)n * HW * C + t.c0 + q * V;
+  if (!on) return;
   float mu[V], rs[V], ga[V], be[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -462,13 +491,12 @@ __global__ __launch_bounds__(512) void gn_apply_kernel(const T* __restrict__ x, 
     ga[e] = gamma ? gamma[c] : 1.f;
     be[e] = beta ? beta[c] : 0.f;
   }
-  walk<8, true>(p, HW, b, l, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); },
-          [&](int64_t i, const Vec<T, V>& r) {
-            float o[V];
+  w.each([&](int64_t i, const Vec<T, V>& r) {
+    float o[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) o[e] = act_fwd<ACT>(fmaf(((float)r.v[e] - mu[e]) * rs[e], ga[e], be[e]), slope);
-            stv<T, V, NT>(ys + i * C, o);
-          });
+    for (int e = 0; e < V; ++e) o[e] = act_fwd<ACT>(fmaf(((float)r.v[e] - mu[e]) * rs[e], ga[e], be[e]), slope);
+    stv<T, V, NT>(ys + i * C, o);
+  });
 }
 
 template <class T, int V>
@@ -493,6 +521,10 @@ __global__ __launch_bounds__(512) void gn_bwd_stats_kernel(const T* __restrict__
   if (on) {
     const T* xs = x + n * xi.ns + t.c0 + q * V;
     const T* ds = dy + n * di.ns + t.c0 + q * V;
+    auto w = walk<false>(p, HW, b, l, [&](int64_t i) {
+      return Two<T, V>{*reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps), *reinterpret_cast<const Vec<T, V>*>(ds + i * di.ps)};
+    });
+    w.begin();
     float mu[V], rs[V], ga[V], be[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -502,11 +534,7 @@ __global__ __launch_bounds__(512) void gn_bwd_stats_kernel(const T* __restrict__
       ga[e] = gamma ? gamma[c] : 1.f;
       be[e] = beta ? beta[c] : 0.f;
     }
-    walk<8, false>(p, HW, b, l,
-            [&](int64_t i) {
-              return Two<T, V>{*reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps), *reinterpret_cast<const Vec<T, V>*>(ds + i * di.ps)};
-            },
-            [&](int64_t, const Two<T, V>& r) {
+    w.each([&](int64_t, const Two<T, V>& r) {
 #pragma unroll
               for (int e = 0; e < V; ++e) {
                 const float xh = ((float)r.x.v[e] - mu[e]) * rs[e];
@@ -601,17 +629,22 @@ __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(const T* __restrict__
   const int block = backwards(blockIdx.x - extra, gridDim.x - extra);
   const Tile t = tile_of<V>(p, block % p.tiles, G);
   const int b = (block / p.tiles) % p.nb, n = block / (p.tiles * p.nb);
+  const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
+  const bool on = l < p.pl && q < t.nq;
+  const T* xs = x + n * xi.ns + t.c0 + q * V;
+  const T* ds = dy + n * di.ns + t.c0 + q * V;
+  T* os = dx + (int64_t)n * HW * C + t.c0 + q * V;
+  auto w = walk<true>(p, HW, b, l, [&](int64_t i) {
+    return Two<T, V>{*reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps), *reinterpret_cast<const Vec<T, V>*>(ds + i * di.ps)};
+  });
+  if (on) w.begin();
   for_groups(t.ng, [&](int g, int lane, int lanes) {
     const int k = t.g0 + min(g, t.ng - 1);
     const float2 r = folded ? part[n * G + k] : fold_means(part, p, HW, G, n, k, lane, lanes);
     if (g < t.ng && lane == 0) stat[g] = r;
   });
   __syncthreads();
-  const int l = threadIdx.x / p.qt, q = threadIdx.x % p.qt;
-  if (l >= p.pl || q >= t.nq) return;
-  const T* xs = x + n * xi.ns + t.c0 + q * V;
-  const T* ds = dy + n * di.ns + t.c0 + q * V;
-  T* os = dx + (int64_t)n * HW * C + t.c0 + q * V;
+  if (!on) return;
   float mu[V], rs[V], ga[V], be[V], c1[V], c2[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -623,20 +656,16 @@ __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(const T* __restrict__
     c1[e] = stat[g].x;
     c2[e] = stat[g].y;
   }
-  walk<4, true>(p, HW, b, l,
-          [&](int64_t i) {
-            return Two<T, V>{*reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps), *reinterpret_cast<const Vec<T, V>*>(ds + i * di.ps)};
-          },
-          [&](int64_t i, const Two<T, V>& r) {
-            float o[V];
+  w.each([&](int64_t i, const Two<T, V>& r) {
+    float o[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const float xh = ((float)r.x.v[e] - mu[e]) * rs[e];
-              const float t1 = (float)r.d.v[e] * act_bwd<ACT>(fmaf(xh, ga[e], be[e]), slope) * ga[e];
-              o[e] = rs[e] * (t1 - c1[e] - xh * c2[e]);
-            }
-            stv<T, V, NT>(os + i * C, o);
-          });
+    for (int e = 0; e < V; ++e) {
+      const float xh = ((float)r.x.v[e] - mu[e]) * rs[e];
+      const float t1 = (float)r.d.v[e] * act_bwd<ACT>(fmaf(xh, ga[e], be[e]), slope) * ga[e];
+      o[e] = rs[e] * (t1 - c1[e] - xh * c2[e]);
+    }
+    stv<T, V, NT>(os + i * C, o);
+  });
 }
 
 // ---------------------------------------------------------------- host side
@@ -645,7 +674,9 @@ inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 constexpr int kMostVectors = 512;      // of a tile: its threads
 constexpr int64_t kMostThreads = (int64_t)1 << 32;   // of a launch
-constexpr int kFoldMost = 4096;        // partial results that a workgroup of the second pass folds by itself
+// Partial results that a workgroup of the second pass folds by itself: 2048 of them beat a launch for it (8x32x1024x64 fp32, the pair:
+// 95 us to 98), 9344 do not (2x32x1024x704 bf16: 164 to 148)
+constexpr int kFoldMost = 4096;
 
 // widest vector that the channels, the strides and every pointer allow
 inline int vector_width(int esize, int C, int G, bool small, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
@@ -687,10 +718,15 @@ inline Plan make_plan(int N, int64_t HW, int C, int G, int V) {
   p.pl = most / p.qt > 1 ? most / p.qt : 1;
   p.threads = (p.qt * p.pl + 63) / 64 * 64;
   // about 1024 workgroups of 256 threads
-  p.runs = (HW + (int64_t)kRun * p.pl - 1) / ((int64_t)kRun * p.pl);
+  p.run = kRun * p.pl;
+  const int64_t runs = (HW + p.run - 1) / p.run;
   int64_t want = 262144 / p.threads / ((int64_t)N * p.tiles);
   want = want < 1 ? 1 : want > 512 ? 512 : want;
-  p.nb = (int)(p.runs < want ? p.runs : want);
+  p.nb = (int)(runs < want ? runs : want);
+  p.each = runs / p.nb;
+  p.more = (int)(runs % p.nb);
+  p.last = (int)((runs - 1) % p.nb);
+  p.missing = (int)(runs * p.run - HW);
   return p;
 }
 

@@ -768,7 +768,7 @@ def _grad_records(grads, kind, what):
     return buf, n, index, _TYPES[types[1]]
 
 
-def _grad_norm(records, max_norm, what):
+def _grad_norm(call, records, max_norm, what):
     if not max_norm >= 0.0:
         raise ValueError(f"{what}: max_norm is not negative, got {max_norm}")
     buf, n, index, ty = records
@@ -776,7 +776,7 @@ def _grad_norm(records, max_norm, what):
     part = torch.empty(L.lib().c3d_grad_norm_partials(buf, n, ty), device=dev, dtype=torch.float64)
     out = torch.empty(2, device=dev, dtype=torch.float32)
     norm, scale = out[0], out[1]
-    _call_on(index, "c3d_grad_norm", buf, n, ty, max_norm, _dp(part), _dp(norm), _dp(scale))
+    _call_on(index, call, buf, n, ty, max_norm, _dp(part), _dp(norm), _dp(scale))
     return norm, scale
 
 
@@ -785,16 +785,12 @@ def grad_norm(grads, max_norm=float("inf")):
     of ``torch.nn.utils.clip_grad_norm_`` -- as 0-dim fp32 device tensors; nothing waits for them.  ``scale`` is what ``adamw_step``
     takes as ``grad_scale``: clipping then costs no pass of its own.  Squares and sums are 64 bits wide.  A gradient that is not
     finite gives a norm that is not finite (and a scale of 0 or NaN), as in torch."""
-    return _grad_norm(_grad_records(grads, "r", "grad_norm"), float(max_norm), "grad_norm")
+    return _grad_norm("c3d_grad_norm", _grad_records(grads, "r", "grad_norm"), float(max_norm), "grad_norm")
 
 
 def clip_grad_norm_(grads, max_norm):
     """Scales a list of gradients in place such that their joint 2-norm is at most ``max_norm``; returns the norm they had."""
-    records = _grad_records(grads, "w", "clip_grad_norm_")
-    norm, scale = _grad_norm(records, float(max_norm), "clip_grad_norm_")
-    buf, n, index, ty = records
-    _call_on(index, "c3d_scale_tensors", buf, n, ty, _dp(scale))
-    return norm
+    return _grad_norm("c3d_clip_grads", _grad_records(grads, "w", "clip_grad_norm_"), float(max_norm), "clip_grad_norm_")[0]
 
 
 def _device_scalar(t, index, what):

@@ -357,11 +357,12 @@ typedef struct {
 /* number of doubles of c3d_grad_norm's workspace (host call)                                                       */
 int64_t c3d_grad_norm_partials(const c3d_opt_tensor* t, int count, int type);
 /* *norm = sqrt(sum of all squares) (sums in 64 bits, fixed order), *scale = min(1, max_norm / (norm + 1e-6)): the factor of
- * torch.nn.utils.clip_grad_norm_, for c3d_scale_tensors or c3d_adamw_desc.grad_scale.  type as above.               */
+ * torch.nn.utils.clip_grad_norm_, for c3d_adamw_desc.grad_scale.  type as above.                                    */
 int c3d_grad_norm(const c3d_opt_tensor* t, int count, int type, double max_norm, double* partial, float* norm,
                   float* scale, c3d_stream stream);
-/* gradient *= *scale, in place                                                                                     */
-int c3d_scale_tensors(const c3d_opt_tensor* t, int count, int type, const float* scale, c3d_stream stream);
+/* the same norm, and every gradient times the factor, in place; *scale is scratch                                  */
+int c3d_clip_grads(const c3d_opt_tensor* t, int count, int type, double max_norm, double* partial, float* norm,
+                   float* scale, c3d_stream stream);
 typedef struct {
   double lr, beta1, beta2, eps, weight_decay;
   const float* grad_scale;   /* device scalar the gradients are multiplied with on load, or NULL                    */
