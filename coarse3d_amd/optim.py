@@ -1,4 +1,6 @@
-"""AdamW over ONE flat parameter / gradient / state buffer.
+"""Optimisers: ``FlatAdamW`` (below), and ``AdamW`` / ``clip_grad_norm_`` over many tensors (their docstrings).
+
+FlatAdamW: AdamW over ONE flat parameter / gradient / state buffer.
 
 The reference builds ``torch.optim.AdamW(model.parameters(), lr)`` (tasks/weak_segmentation/trainer.py:146-151: one
 parameter group, default betas / eps / weight decay on every tensor).  With one group the update is the same elementwise
@@ -25,8 +27,13 @@ in ``model.parameters()`` order (197 for SalsaNextProto: the frozen ``prototypes
 ``mask_norm.*`` are 193-196), and ``state`` holds entries for the parameters that have been stepped."""
 import torch
 
+from . import ops
+from .ops import grad_norm
+
 
 class FlatAdamW(torch.optim.Optimizer):
+    graph_safe = True            # TrainStep(graph=True) may capture the update
+
     def __init__(self, named_params, grad_views, flat_grad, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                  all_params=None):
         """named_params: (name, parameter) of the parameters that live in the flat buffers, in buffer order.
@@ -221,3 +228,274 @@ class FlatAdamW(torch.optim.Optimizer):
             self._segments = segs
         for g, s in zip(self.param_groups, sd["param_groups"]):
             g.update({k: v for k, v in s.items() if k != "params"})
+
+
+class _Cohort:
+    """Parameters that have always been stepped together, and how often."""
+    __slots__ = ("step", "step_t")
+
+    def __init__(self, step=0, step_t=None):
+        self.step, self.step_t = step, step_t
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over any list of parameters on the many-tensor kernels (``ops.adamw_step`` / ``ops.adamw8_step``): the formula, the
+    argument names and -- with 32-bit states -- the checkpoint layout of ``torch.optim.AdamW``, parameter groups, schedulers
+    and parameters without a gradient (skipped, as torch skips them) included.  Beside ``FlatAdamW``, which steps ONE flat buffer
+    through torch's kernel, it takes parameters where they are and adds what training on one or two scans per GPU asks for:
+
+    ``state_bits=8``: both moments in 8 bits (e4m3 times a power of two for every 256 elements, rounded stochastically from ``seed``
+        and the step count): 2 bytes a parameter instead of 8, and 16 instead of 28 bytes moved a step.
+    ``master_weights=True``: 16-bit parameters are stepped as fp32 copies in the state and written from them.
+    ``max_grad_norm``: the gradients are clipped by their global norm on load -- one pass over them, no write; ``last_grad_norm``
+        is that norm (a device scalar, before clipping).
+    ``capturable=True``: step counts and learning rates live on the device (all parameters on one), for a captured step
+        (``TrainStep(graph=True)``); ``sync_lr()`` copies changed learning rates, ``generation`` counts what makes a captured step
+        stale.  As with every optimiser, the first steps of a configuration have to run outside the capture."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, master_weights=False,
+                 max_grad_norm=None, capturable=False, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits is 8 or 32, got {state_bits}")
+        if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"AdamW: lr, eps and weight_decay are not negative and betas in [0, 1); got {lr}, {eps}, {weight_decay}, {betas}")
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError(f"AdamW: max_grad_norm is not negative, got {max_grad_norm}")
+        self.state_bits, self.master_weights, self.max_grad_norm = state_bits, master_weights, max_grad_norm
+        self.capturable, self.seed = capturable, seed
+        self.last_grad_norm = None
+        self.generation = 0
+        self._cohort_of = {}             # id(parameter) -> _Cohort
+        self._plan = None                # (which parameters have a gradient, [launch lists]) of the last step
+        self._lr_t = {}                  # group index -> (value seen, device scalar)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    @property
+    def graph_safe(self):
+        """Whether ``TrainStep(graph=True)`` may capture the update."""
+        return self.capturable
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        self._plan = None
+
+    # ------------------------------------------------------------------ state
+    def _init_state(self, p):
+        like = lambda dtype: torch.empty_like(p, dtype=dtype).zero_()  # noqa: E731
+        st = self.state[p]
+        if self.state_bits == 8:
+            blocks = (p.numel() + ops.ADAMW8_BLOCK - 1) // ops.ADAMW8_BLOCK
+            for name in ("exp_avg", "exp_avg_root"):
+                st[name] = like(torch.uint8).view(torch.float8_e4m3fn)
+                st[name + "_scale"] = torch.zeros(blocks, device=p.device, dtype=torch.float32)
+        else:
+            st["exp_avg"], st["exp_avg_sq"] = like(torch.float32), like(torch.float32)
+        if self.master_weights and p.dtype != torch.float32:
+            st["master"] = p.detach().float()
+
+    _STATE = {32: ("exp_avg", "exp_avg_sq", None, None), 8: ("exp_avg", "exp_avg_root", "exp_avg_scale", "exp_avg_root_scale")}
+
+    def _split_cohorts(self, params, grads):
+        """Give every parameter with a gradient a cohort of parameters that all have one; new parameters get their state."""
+        first, halves, capturing = None, {}, None
+        for p, g in zip(params, grads):
+            if g is None:
+                continue
+            if p not in self.state or not self.state[p]:
+                capturing = torch.cuda.is_current_stream_capturing() if capturing is None and p.is_cuda else capturing
+                if capturing:
+                    raise RuntimeError("AdamW: a parameter is stepped for the first time inside a graph capture; run an eager step in "
+                                       "this configuration first")
+                if g.is_sparse:
+                    raise RuntimeError("AdamW: sparse gradients are not supported")
+                self._init_state(p)
+                if first is None:
+                    first = _Cohort(0, torch.zeros((), device=p.device, dtype=torch.float32) if self.capturable else None)
+                    self.generation += 1
+                self._cohort_of[id(p)] = first
+        # a cohort of which only some have a gradient: those get a counter of their own
+        idle = {id(self._cohort_of[id(p)]) for p, g in zip(params, grads) if g is None and id(p) in self._cohort_of}
+        if not idle:
+            return
+        for p, g in zip(params, grads):
+            c = self._cohort_of.get(id(p))
+            if g is not None and id(c) in idle:
+                if id(c) not in halves:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("AdamW: the set of parameters with a gradient changed inside a graph capture; run an eager "
+                                           "step in this configuration first")
+                    halves[id(c)] = _Cohort(c.step, c.step_t.clone() if c.step_t is not None else None)
+                    self.generation += 1
+                self._cohort_of[id(p)] = halves[id(c)]
+
+    def _launches(self, grads_by_group):
+        """[(group index, cohort, parameter indices, params, [state lists], masters)] of parameters with a gradient: one entry for each
+        group, step count, device and type."""
+        runs = {}
+        for gi, (group, grads) in enumerate(zip(self.param_groups, grads_by_group)):
+            for i, (p, g) in enumerate(zip(group["params"], grads)):
+                if g is not None:
+                    master = "master" in self.state[p]
+                    runs.setdefault((gi, id(self._cohort_of[id(p)]), p.device, p.dtype, g.dtype, master), []).append(i)
+        out = []
+        for (gi, _, _, _, _, master), idx in runs.items():
+            ps = [self.param_groups[gi]["params"][i] for i in idx]
+            states = [None if name is None else [self.state[p][name] for p in ps] for name in self._STATE[self.state_bits]]
+            out.append((gi, self._cohort_of[id(ps[0])], idx, ps, states, [self.state[p]["master"] for p in ps] if master else None))
+        return out
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        grads = [[p.grad for p in g["params"]] for g in self.param_groups]
+        active = [[None if x is None else x.dtype for x in g] for g in grads]
+        if self._plan is None or self._plan[0] != active:
+            self._split_cohorts([p for g in self.param_groups for p in g["params"]], [x for g in grads for x in g])
+            self._plan = (active, self._launches(grads))
+        launches = self._plan[1]
+        if not launches:
+            return loss
+        capturing = launches[0][3][0].is_cuda and torch.cuda.is_current_stream_capturing()
+        if self.capturable:
+            if len({p.device for run in launches for p in run[3][:1]}) > 1:
+                raise RuntimeError("AdamW(capturable=True): the parameters are on several devices")
+            if not capturing:
+                self.sync_lr()
+        lists = [[grads[gi][i] for i in idx] for gi, _, idx, _, _, _ in launches]
+        scale = None
+        if self.max_grad_norm is not None:
+            scale = self._clip_factor(lists)
+        for c in {id(run[1]): run[1] for run in launches}.values():
+            c.step += 1
+            if c.step_t is not None:
+                c.step_t.add_(1.0)
+        for (gi, cohort, _, ps, states, masters), gs in zip(launches, lists):
+            group = self.param_groups[gi]
+            more = dict(step=cohort.step_t if self.capturable else cohort.step, lr=self._lr_t[gi][1] if self.capturable else float(group["lr"]),
+                        betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=scale, masters=masters)
+            try:
+                self._launch(gi, ps, gs, states, more)
+            except ValueError:          # (refused before anything was launched) a gradient in another memory layout than its parameter
+                if all(g.stride() == p.stride() for g, p in zip(gs, ps)):
+                    raise
+                self._launch(gi, ps, [torch.empty_like(p, dtype=g.dtype).copy_(g) for g, p in zip(gs, ps)], states, more)
+        return loss
+
+    def _launch(self, gi, params, grads, states, more):
+        m, v, ms, vs = states
+        if self.state_bits == 8:
+            ops.adamw8_step(params, grads, m, ms, v, vs, seed=self.seed + gi, **more)
+        else:
+            ops.adamw_step(params, grads, m, v, **more)
+
+    def _clip_factor(self, lists):
+        by_type = {}
+        for gs in lists:
+            by_type.setdefault(gs[0].dtype, []).extend(gs)
+        if len(by_type) == 1:
+            self.last_grad_norm, scale = grad_norm(next(iter(by_type.values())), self.max_grad_norm)
+            return scale
+        norms = torch.stack([grad_norm(gs)[0] for gs in by_type.values()]).double()
+        total = norms.square().sum().sqrt()
+        self.last_grad_norm = total.float()
+        return torch.clamp(self.max_grad_norm / (total + 1e-6), max=1.0).float()
+
+    def sync_lr(self):
+        """Copy learning rates that schedulers have changed into the device scalars of a capturable optimiser."""
+        if not self.capturable:
+            return
+        for gi, group in enumerate(self.param_groups):
+            lr = float(group["lr"])
+            seen = self._lr_t.get(gi)
+            if seen is None:
+                if not group["params"]:
+                    continue
+                self._lr_t[gi] = (lr, torch.full((), lr, device=group["params"][0].device, dtype=torch.float32))
+            elif seen[0] != lr:
+                seen[1].fill_(lr)
+                self._lr_t[gi] = (lr, seen[1])
+
+    # ------------------------------------------------------------------ checkpoints
+    def _step_of(self, p):
+        c = self._cohort_of.get(id(p))
+        return 0.0 if c is None else float(c.step_t) if c.step_t is not None else float(c.step)
+
+    def state_dict(self):
+        """torch's layout: ``state[i]`` of the i-th parameter over all groups, with its own ``step``; ``state_bits`` stands beside it."""
+        groups, index, at = [], {}, 0
+        for g in self.param_groups:
+            groups.append(dict({k: v for k, v in g.items() if k != "params"}, params=list(range(at, at + len(g["params"])))))
+            for p in g["params"]:
+                index[id(p)] = at
+                at += 1
+        state = {index[id(p)]: dict({"step": torch.tensor(self._step_of(p))}, **{k: v.detach().clone() for k, v in st.items()})
+                 for p, st in self.state.items() if st}
+        return {"state": state, "param_groups": groups, "state_bits": self.state_bits}
+
+    @torch.no_grad()
+    def load_state_dict(self, sd):
+        """Checkpoints of this class with the same ``state_bits``, and of ``torch.optim.AdamW`` with 32."""
+        if len(sd["param_groups"]) != len(self.param_groups) or any(
+                len(a["params"]) != len(b["params"]) for a, b in zip(sd["param_groups"], self.param_groups)):
+            raise ValueError("AdamW.load_state_dict: the checkpoint's parameter groups differ from this optimiser's")
+        params = {}
+        for a, b in zip(sd["param_groups"], self.param_groups):
+            params.update(zip(a["params"], b["params"]))
+        names = [n for n in self._STATE[self.state_bits] if n is not None]
+        new = {}
+        for key, st in sd["state"].items():
+            p = params.get(key)
+            if p is None or not set(names) <= set(st) or "step" not in st:
+                raise ValueError(f"AdamW.load_state_dict: state {key} is not that of a parameter with {self.state_bits}-bit states")
+            mine = {}
+            for n in names + (["master"] if "master" in st else []):
+                t = st[n]
+                blocks = n.endswith("_scale")
+                if (t.numel() != (p.numel() + ops.ADAMW8_BLOCK - 1) // ops.ADAMW8_BLOCK) if blocks else t.shape != p.shape:
+                    raise ValueError(f"AdamW.load_state_dict: {n} of state {key} does not fit its parameter")
+                if self.state_bits == 8 and not blocks and n != "master":
+                    if t.dtype != torch.float8_e4m3fn:
+                        raise ValueError(f"AdamW.load_state_dict: {n} of state {key} is {t.dtype}, not float8_e4m3fn")
+                    # (codes belong to blocks of memory: the layout has to be the checkpoint's, or the parameter's where both are dense alike)
+                    if t.stride() != p.stride():
+                        raise ValueError(f"AdamW.load_state_dict: {n} of state {key} has another memory layout than its parameter")
+                    mine[n] = torch.empty_like(p, dtype=torch.uint8).copy_(t.view(torch.uint8)).view(torch.float8_e4m3fn)
+                elif blocks:
+                    mine[n] = t.detach().to(device=p.device, dtype=torch.float32, copy=True).reshape(-1).contiguous()
+                else:
+                    mine[n] = torch.empty_like(p, dtype=torch.float32).copy_(t)
+            if self.master_weights and p.dtype != torch.float32 and "master" not in mine:
+                mine["master"] = p.detach().float()
+            if not self.master_weights:
+                mine.pop("master", None)
+            new[p] = (mine, float(st["step"]))
+        cohorts = {}
+        self.state.clear()
+        self._cohort_of.clear()
+        for p, (mine, t) in new.items():
+            self.state[p] = mine
+            if (t, p.device) not in cohorts:
+                cohorts[t, p.device] = _Cohort(int(t), torch.full((), t, device=p.device, dtype=torch.float32) if self.capturable else None)
+            self._cohort_of[id(p)] = cohorts[t, p.device]
+        for g, s in zip(self.param_groups, sd["param_groups"]):
+            g.update({k: tuple(v) if k == "betas" else v for k, v in s.items() if k in ("lr", "betas", "eps", "weight_decay", "initial_lr")})
+        self._plan = None
+        self.generation += 1
+
+
+def clip_grad_norm_(parameters, max_norm):
+    """``torch.nn.utils.clip_grad_norm_`` on the many-tensor kernels: scales the gradients of ``parameters`` in place such that their
+    joint 2-norm is at most ``max_norm``; returns the norm they had, as a device scalar that nothing waits for."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    by_type = {}
+    for p in params:
+        if p.grad is not None:
+            by_type.setdefault(p.grad.dtype, []).append(p.grad)
+    if not by_type:
+        return torch.zeros((), device=params[0].device if params else None)
+    if len(by_type) == 1:
+        return ops.clip_grad_norm_(next(iter(by_type.values())), max_norm)
+    raise ValueError(f"clip_grad_norm_: the gradients have several types: {sorted(map(str, by_type))}")

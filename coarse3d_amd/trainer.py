@@ -286,9 +286,10 @@ class TrainStep:
             return ("the HIP runtime was initialised before `import coarse3d_amd` without DEBUG_CLR_GRAPH_PACKET_CAPTURE=0: a "
                     "captured step would fault when replayed after ~2 000 unrelated launches (coarse3d_amd/__init__.py).  Import "
                     "coarse3d_amd before the first torch.cuda call, export the variable, or set C3D_GRAPH_UNSAFE=1 to capture anyway")
-        if type(self.optimizer).__name__ != "FlatAdamW":
+        if not getattr(self.optimizer, "graph_safe", False):
             return ("the captured step needs the flat optimiser (coarse3d_amd.optim.FlatAdamW: learning rate as a device "
-                    "scalar, gradient-less parameters skipped); a user-supplied optimiser runs with graph=False")
+                    "scalar, gradient-less parameters skipped) or coarse3d_amd.optim.AdamW(capturable=True); any other user-supplied "
+                    "optimiser runs with graph=False")
         return None
 
     def _sync_ratio(self, epoch):
