@@ -83,9 +83,8 @@ def native():
         except ImportError as e:
             raise RuntimeError("coarse3d_amd/_native.so is missing or does not load: the extension has not been built (run "
                                "`python -c 'import __graft_entry__ as g; g.build()'`). There is no fallback.") from e
-        address = lambda f: C.cast(f, C.c_void_p).value  # noqa: E731
         k = lib()
-        _native.bind(address(k.c3d_group_norm), address(k.c3d_group_norm_bwd), address(k.c3d_group_norm_ws_floats), address(k.c3d_last_error))
+        _native.bind({n: C.cast(getattr(k, n), C.c_void_p).value for n in prototypes() if hasattr(k, n)})
         _nat = _native
     return _nat
 

@@ -715,28 +715,16 @@ def sums_to_f32(sums, col, out, accumulate=False):
     return out
 
 
-def _call_on(index, name, *args):
-    """``_call`` on the device that the tensors live on, on that device's current stream."""
-    if index == _cur_dev():
-        _call(name, *args, _stream())
-    else:
-        with torch.cuda.device(index):
-            _call(name, *args, _stream())
-
-
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
 # ---------------------------------------------------------------------------- GroupNorm with an activation
 def _on_device_of(x, call, *args):
-    """call(*args, stream) with x's device current; a tensor elsewhere than on a GPU is left for the call to refuse."""
-    index = x.get_device()
+    """call(*args, stream) with tensor x's device current, on its current stream; what is not on a GPU is left for the call to refuse."""
+    index = x.get_device() if isinstance(x, torch.Tensor) else -1
     if index < 0:
         return call(*args, 0)
-    if index == _cur_dev():
-        return call(*args, _stream().value or 0)
+    if index == torch._C._cuda_getDevice():           # (a tensor on a GPU: the runtime is up)
+        return call(*args, _raw_stream(index))
     with torch.cuda.device(index):
-        return call(*args, _stream().value or 0)
+        return call(*args, _raw_stream(index))
 
 
 def group_norm(x, groups, gamma=None, beta=None, eps=1e-5, act="lrelu", slope=0.01):
@@ -756,28 +744,10 @@ def group_norm_bwd(dy, x, mean, rstd, gamma=None, beta=None, act="lrelu", slope=
 
 # ---------------------------------------------------------------------------- optimiser over many tensors
 ADAMW8_BLOCK = 256       # elements of an 8-bit state that share a scale (C3D_ADAMW8_BLOCK)
-_GRAD_NAMES = ("", "grads", "", "", "", "", "")
 
 
-def _grad_records(grads, kind, what):
-    buf, n, index, types = L.native().pack(what, (None, grads, None, None, None, None, None), "w" + kind + "wwwww", _GRAD_NAMES)
-    if n == 0:
-        raise ValueError(f"{what}: no tensors")
-    if types[1] not in _TYPES:
-        raise ValueError(f"{what}: gradients are fp32, bf16 or fp16, got {types[1]}")
-    return buf, n, index, _TYPES[types[1]]
-
-
-def _grad_norm(call, records, max_norm, what):
-    if not max_norm >= 0.0:
-        raise ValueError(f"{what}: max_norm is not negative, got {max_norm}")
-    buf, n, index, ty = records
-    dev = torch.device("cuda", index)
-    part = torch.empty(L.lib().c3d_grad_norm_partials(buf, n, ty), device=dev, dtype=torch.float64)
-    out = torch.empty(2, device=dev, dtype=torch.float32)
-    norm, scale = out[0], out[1]
-    _call_on(index, call, buf, n, ty, max_norm, _dp(part), _dp(norm), _dp(scale))
-    return norm, scale
+def _first(tensors):
+    return tensors[0] if isinstance(tensors, (list, tuple)) and tensors else None
 
 
 def grad_norm(grads, max_norm=float("inf")):
@@ -785,64 +755,18 @@ def grad_norm(grads, max_norm=float("inf")):
     of ``torch.nn.utils.clip_grad_norm_`` -- as 0-dim fp32 device tensors; nothing waits for them.  ``scale`` is what ``adamw_step``
     takes as ``grad_scale``: clipping then costs no pass of its own.  Squares and sums are 64 bits wide.  A gradient that is not
     finite gives a norm that is not finite (and a scale of 0 or NaN), as in torch."""
-    return _grad_norm("c3d_grad_norm", _grad_records(grads, "r", "grad_norm"), float(max_norm), "grad_norm")
+    return _on_device_of(_first(grads), L.native().grad_norm, "grad_norm", grads, max_norm, False)
 
 
 def clip_grad_norm_(grads, max_norm):
     """Scales a list of gradients in place such that their joint 2-norm is at most ``max_norm``; returns the norm they had."""
-    return _grad_norm("c3d_clip_grads", _grad_records(grads, "w", "clip_grad_norm_"), float(max_norm), "clip_grad_norm_")[0]
-
-
-def _device_scalar(t, index, what):
-    if t.numel() != 1 or t.dtype != torch.float32 or t.get_device() != index:
-        raise ValueError(f"{what} as a tensor is one fp32 value on the parameters' device")
-    return t.data_ptr()
-
-
-def _adamw(what, lists, kinds, names, bits, step, lr, betas, eps, weight_decay, grad_scale, seed):
-    buf, n, index, types = L.native().pack(what, lists, kinds, names)
-    if n == 0:
-        raise ValueError(f"{what}: no tensors")
-    p, g, m, v, ms, vs, w = types
-    if p not in _TYPES or g not in (p, torch.float32):
-        raise ValueError(f"{what}: parameters are fp32, bf16 or fp16 and gradients of the same type or fp32, got {p} and {g}")
-    want = torch.float32 if bits == 32 else torch.float8_e4m3fn
-    if m != want or v != want:
-        raise ValueError(f"{what}: the states are {want}, got {m} and {v}")
-    if bits == 8 and (ms != torch.float32 or vs != torch.float32):
-        raise ValueError(f"{what}: the states' scales are fp32, got {ms} and {vs}")
-    if w is not None and (w != torch.float32 or p == torch.float32):
-        raise ValueError(f"{what}: master copies are fp32, of 16-bit parameters; got {w} of {p}")
-    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
-        raise ValueError(f"{what}: betas are in [0, 1), got {betas}")
-    if not eps >= 0.0:
-        raise ValueError(f"{what}: eps is not negative, got {eps}")
-    d = L.AdamWDesc()
-    if isinstance(lr, torch.Tensor):
-        d.lr_dev = _device_scalar(lr, index, f"{what}: lr")
-    else:
-        d.lr = lr
-    if isinstance(step, torch.Tensor):
-        d.step_dev = _device_scalar(step, index, f"{what}: step")
-    elif step < 1:
-        raise ValueError(f"{what}: step counts from 1, got {step}")
-    else:
-        d.step = step
-    if grad_scale is not None:
-        d.grad_scale = _device_scalar(grad_scale, index, f"{what}: grad_scale")
-    d.beta1, d.beta2, d.eps, d.weight_decay = betas[0], betas[1], eps, weight_decay
-    d.param_type, d.grad_type, d.state_bits, d.has_master, d.seed = _TYPES[p], _TYPES[g], bits, int(w is not None), seed & 0xFFFFFFFF
-    _call_on(index, "c3d_adamw_step", buf, n, C.byref(d))
-
-
-_ADAMW_NAMES = ("params", "grads", "exp_avgs", "exp_avg_sqs", "", "", "masters")
-_ADAMW8_NAMES = ("params", "grads", "exp_avgs", "exp_avg_roots", "exp_avg_scales", "exp_avg_root_scales", "masters")
+    return _on_device_of(_first(grads), L.native().grad_norm, "clip_grad_norm_", grads, max_norm, True)[0]
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, grad_scale=None,
                masters=None):
     """One AdamW step (torch.optim.AdamW's formula) over lists of tensors, in place, in as few launches as the kernel arguments
-    allow (88 tensors each; 72 with masters).
+    allow (about 160 tensors each).
 
     params fp32, bf16 or fp16, one type a call; grads of that type or fp32; exp_avgs / exp_avg_sqs fp32; masters: fp32 copies of
     16-bit parameters, which then carry the value (the parameter is written from them, rounded to nearest) -- without them an update
@@ -850,8 +774,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
     layout, whatever the order of their dimensions; sizes from zero.  No two written tensors may share memory.
     step: 1 for the first step, or, like lr, a 0-dim fp32 device tensor read when the kernel runs (a captured step).
     grad_scale: 0-dim fp32 device tensor the gradients are multiplied with on load (``grad_norm``)."""
-    _adamw("adamw_step", (params, grads, exp_avgs, exp_avg_sqs, None, None, masters), "wrwwssw", _ADAMW_NAMES, 32, step, lr, betas, eps,
-           weight_decay, grad_scale, 0)
+    _on_device_of(_first(params), L.native().adamw, "adamw_step", (params, grads, exp_avgs, exp_avg_sqs, None, None, masters), 32, step, lr,
+                  betas[0], betas[1], eps, weight_decay, grad_scale, 0)
 
 
 def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_roots, exp_avg_root_scales, *, step, lr, betas=(0.9, 0.999), eps=1e-8,
@@ -861,8 +785,9 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_roots, exp_avg_
     zeros.  The step itself is computed in fp32 from the states' values; what is stored is rounded stochastically -- in the mean
     exact, so that a change of 0.1 % a step is not lost -- with bits that depend on (seed, step, place in the lists) and nothing
     else.  A root above zero never becomes zero; an element that is not finite becomes NaN and leaves its neighbours alone."""
-    _adamw("adamw8_step", (params, grads, exp_avgs, exp_avg_roots, exp_avg_scales, exp_avg_root_scales, masters), "wrwwssw", _ADAMW8_NAMES, 8,
-           step, lr, betas, eps, weight_decay, grad_scale, seed)
+    _on_device_of(_first(params), L.native().adamw, "adamw8_step",
+                  (params, grads, exp_avgs, exp_avg_roots, exp_avg_scales, exp_avg_root_scales, masters), 8, step, lr, betas[0], betas[1], eps,
+                  weight_decay, grad_scale, seed & 0xFFFFFFFF)
 
 
 # ---------------------------------------------------------------------------- glue
