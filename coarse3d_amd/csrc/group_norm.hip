@@ -722,6 +722,9 @@ inline Plan make_plan(int N, int64_t HW, int C, int G, int V) {
   const int64_t runs = (HW + p.run - 1) / p.run;
   int64_t want = 262144 / p.threads / ((int64_t)N * p.tiles);
   want = want < 1 ? 1 : want > 512 ? 512 : want;
+  // (at most 64 runs each, so that no fp32 sum of a thread has more than 256 terms)
+  const int64_t least = (runs + 63) / 64;
+  want = want < least ? least : want;
   p.nb = (int)(runs < want ? runs : want);
   p.each = runs / p.nb;
   p.more = (int)(runs % p.nb);

@@ -18,13 +18,13 @@ namespace {
 constexpr int kThreads = 256, kNormThreads = 512;
 constexpr int kBlock = C3D_ADAMW8_BLOCK;   // elements a wave of the step handles at a time (four a lane), and that share a scale
 constexpr int64_t kMaxRecord = 1 << 30;    // longer tensors are cut into several records: 32-bit indices inside one
-constexpr uint32_t kMaxBlocks = 1u << 26;  // blocks a launch: its threads stay below 2^32
+constexpr uint32_t kMaxBlocks = 1u << 25;  // blocks a launch: its threads stay below 2^32
 constexpr uint32_t kUnaligned = 1u << 31;
 // Blocks a wave has in flight together.  Short waves: there are several generations of them on a CU, so that some load while others
 // compute; with twice or four times as many blocks a wave all of them ran in step (9.4 M parameters, 8-bit states: 48 us with 1,
 // 51 with 2, 66 with 4; 32-bit ones with the norm: 74, 74, 80).  The norm and the scaling, which compute nothing, want 4 KB a wave
 // (38 MB: 30 us with 4 KB, 31 with 2, 33 with 8).
-constexpr int kStepBlocks = 2, kStep8Blocks = 1, kNormBlocks = 4, kScaleBlocks = 2;
+constexpr int kStepBlocks = 2, kStep8Blocks = 1, kNormBlocks = 4, kScaleBlocks = 2, kSmallBlocks = 4;
 
 // The tensors of a launch, as one sequence of blocks: workgroups are dealt blocks and not tensors, so that a hundred biases of 32
 // elements cost a hundred waves' loads and not a hundred workgroups.
@@ -217,6 +217,55 @@ __global__ __launch_bounds__(1024) void grad_norm_fold_kernel(const double* __re
     const double r = sqrt(s), f = max_norm / (r + 1e-6);
     *norm = (float)r;
     *scale = (float)(f > 1.0 ? 1.0 : f);          // a norm that is not a number stays visible in the factor
+  }
+}
+
+// Everything in one workgroup and one launch, where all values fit its registers: each wave holds kSmallBlocks blocks of 16 bytes a
+// lane.  (Clipping 16 K values: 7 us, 12 in three launches; with four times the blocks a wave it loses, 18 us.)
+template <class T, bool CLIP>
+__global__ __launch_bounds__(1024) void grad_small_kernel(GradTable t, double max_norm, float* __restrict__ norm, float* __restrict__ scale) {
+  constexpr int V = kLane<T>, B = kRun<T>;
+  __shared__ double red[16];
+  const uint32_t lane = threadIdx.x & 63, wave = wave_id();
+  Vec<T, V> x[kSmallBlocks];
+  double s = 0.0;
+#pragma unroll
+  for (int u = 0; u < kSmallBlocks; ++u) {
+    const uint32_t j = u * 16 + wave;
+#pragma unroll
+    for (int q = 0; q < V; ++q) x[u].v[q] = (T)0;
+    if (j < t.blocks) {
+      const int k = find_record(t, j);
+      const uint32_t n = t.n[k] & ~kUnaligned, b = j - t.first[k], i = b * B + lane * V;
+      if (!(t.n[k] & kUnaligned) && (b + 1) * B <= n) x[u] = loadv<true, T, V>(t.at(0, k), i, n);
+      else x[u] = loadv<false, T, V>(t.at(0, k), i, n);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kSmallBlocks; ++u)
+#pragma unroll
+    for (int q = 0; q < V; ++q) s = fma((double)(float)x[u].v[q], (double)(float)x[u].v[q], s);
+  s = group_sum<1024>(s, red);
+  const double r = sqrt(s), f = max_norm / (r + 1e-6);
+  const float factor = (float)(f > 1.0 ? 1.0 : f);
+  if (threadIdx.x == 0) {
+    *norm = (float)r;
+    *scale = factor;
+  }
+  if constexpr (CLIP) {
+#pragma unroll
+    for (int u = 0; u < kSmallBlocks; ++u) {
+      const uint32_t j = u * 16 + wave;
+      if (j < t.blocks) {
+        const int k = find_record(t, j);
+        const uint32_t n = t.n[k] & ~kUnaligned, b = j - t.first[k], i = b * B + lane * V;
+        float o[V];
+#pragma unroll
+        for (int q = 0; q < V; ++q) o[q] = (float)x[u].v[q] * factor;
+        if (!(t.n[k] & kUnaligned) && (b + 1) * B <= n) storev<true, T, V>(t.at(0, k), i, n, o);
+        else storev<false, T, V>(t.at(0, k), i, n, o);
+      }
+    }
   }
 }
 
@@ -652,6 +701,23 @@ int for_each_grad_table(const c3d_opt_tensor* t, int count, int blocks_a_group, 
   return for_each_table<GradTable>(t, count, {{1, (int)sizeof(T)}}, kRun<T>, blocks_a_group, launch);
 }
 constexpr int kNormGroup = kNormBlocks * kNormThreads / 64, kScaleGroup = kScaleBlocks * kThreads / 64;
+// the whole list in one table and in one workgroup's registers?
+template <class T>
+bool is_small(const c3d_opt_tensor* t, int count) {
+  static_assert(16 * kSmallBlocks <= GradTable::kMost, "a tensor has a block at least");
+  int64_t blocks = 0;
+  for (int i = 0; i < count && blocks <= 16 * kSmallBlocks; ++i) blocks += (t[i].n + kRun<T> - 1) / kRun<T>;
+  return blocks > 0 && blocks <= 16 * kSmallBlocks;
+}
+template <class T>
+int small(const c3d_opt_tensor* t, int count, bool clip, double max_norm, float* norm, float* scale, hipStream_t s) {
+  return for_each_grad_table<T>(t, count, 16 * kSmallBlocks, [&](const GradTable& tab, uint32_t) {
+    const auto kernel = clip ? grad_small_kernel<T, true> : grad_small_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), 0, s, tab, max_norm, norm, scale);
+    C3D_CHECK_LAUNCH();
+    return 0;
+  });
+}
 template <class T>
 int sumsq(const c3d_opt_tensor* t, int count, double* partial, hipStream_t s) {
   return for_each_grad_table<T>(t, count, kNormGroup, [&](const GradTable& tab, uint32_t groups) {
@@ -713,6 +779,7 @@ extern "C" int c3d_opt_abi_sizes(int32_t* out2) {
 }
 
 extern "C" int64_t c3d_grad_norm_partials(const c3d_opt_tensor* t, int count, int type) {
+  if (type == 0 ? is_small<float>(t, count) : is_small<_Float16>(t, count)) return 0;
   int64_t parts = 0;
   auto add = [&](const GradTable&, uint32_t groups) {
     parts += groups;
@@ -726,6 +793,14 @@ extern "C" int64_t c3d_grad_norm_partials(const c3d_opt_tensor* t, int count, in
 namespace {
 int sumsq_any(const c3d_opt_tensor* t, int count, int type, double* partial, hipStream_t s) {
   return type == 0 ? sumsq<float>(t, count, partial, s) : type == 1 ? sumsq<__bf16>(t, count, partial, s) : sumsq<_Float16>(t, count, partial, s);
+}
+int small_any(const c3d_opt_tensor* t, int count, int type, bool clip, double max_norm, float* norm, float* scale, hipStream_t s) {
+  return type == 0   ? small<float>(t, count, clip, max_norm, norm, scale, s)
+         : type == 1 ? small<__bf16>(t, count, clip, max_norm, norm, scale, s)
+                     : small<_Float16>(t, count, clip, max_norm, norm, scale, s);
+}
+bool any(const c3d_opt_tensor* t, int count) {
+  return std::any_of(t, t + count, [](const c3d_opt_tensor& x) { return x.n > 0; });
 }
 int fold(const double* partial, int64_t parts, double max_norm, float* norm, float* scale, hipStream_t s) {
   hipLaunchKernelGGL(grad_norm_fold_kernel, dim3(1), dim3(1024), 0, s, partial, parts, max_norm, norm, scale);
@@ -748,6 +823,7 @@ extern "C" int c3d_grad_norm(const c3d_opt_tensor* t, int count, int type, doubl
   if (int rc = check_norm(t, count, type, max_norm, partial, parts)) return rc;
   C3D_REQUIRE(norm && scale, "grad_norm: null output");
   hipStream_t s = (hipStream_t)stream;
+  if (parts == 0 && any(t, count)) return small_any(t, count, type, false, max_norm, norm, scale, s);
   if (int rc = sumsq_any(t, count, type, partial, s)) return rc;
   return fold(partial, parts, max_norm, norm, scale, s);
 }
@@ -758,6 +834,7 @@ extern "C" int c3d_clip_grads(const c3d_opt_tensor* t, int count, int type, doub
   if (int rc = check_norm(t, count, type, max_norm, partial, parts)) return rc;
   C3D_REQUIRE(norm && scale, "clip_grads: null output");
   hipStream_t s = (hipStream_t)stream;
+  if (parts == 0 && any(t, count)) return small_any(t, count, type, true, max_norm, norm, scale, s);
   if (int rc = sumsq_any(t, count, type, partial, s)) return rc;
   if (int rc = fold(partial, parts, max_norm, norm, scale, s)) return rc;
   return type == 0 ? scale_all<float>(t, count, scale, s) : type == 1 ? scale_all<__bf16>(t, count, scale, s) : scale_all<_Float16>(t, count, scale, s);

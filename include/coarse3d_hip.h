@@ -354,7 +354,7 @@ typedef struct {
 } c3d_opt_tensor;
 /* elements that share one scale of an 8-bit state                                                                 */
 #define C3D_ADAMW8_BLOCK 256
-/* number of doubles of c3d_grad_norm's workspace (host call)                                                       */
+/* number of doubles of c3d_grad_norm's workspace, 0 for short lists, which need none (host call)                   */
 int64_t c3d_grad_norm_partials(const c3d_opt_tensor* t, int count, int type);
 /* *norm = sqrt(sum of all squares) (sums in 64 bits, fixed order), *scale = min(1, max_norm / (norm + 1e-6)): the factor of
  * torch.nn.utils.clip_grad_norm_, for c3d_adamw_desc.grad_scale.  type as above.                                    */

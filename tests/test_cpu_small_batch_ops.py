@@ -115,6 +115,7 @@ def test_the_library_refuses_what_the_wrappers_would_not_send():
     rec[0].n = 8
     rec[0].ptr[1] = 16
     assert lib.c3d_grad_norm(rec, 1, 3, 1.0, 8, 8, 8, None) == 2 and lib.c3d_grad_norm(rec, 1, 0, float("nan"), 8, 8, 8, None) == 2
+    rec[0].n = 1 << 20
     assert lib.c3d_grad_norm(rec, 1, 0, 1.0, None, 8, 8, None) == 2 and lib.c3d_clip_grads(rec, 1, 0, 1.0, None, 8, 8, None) == 2
     gn = lambda **k: lib.c3d_group_norm(*dict(dict(x=16, ns=24, ps=8, N=2, HW=3, C=8, G=2, type=0, ga=None, be=None, eps=1e-5, act=1, slope=0.01, y=16,  # noqa: E731
                                                    mean=16, rstd=16, ws=16, s=None), **k).values())

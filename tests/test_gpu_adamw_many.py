@@ -368,25 +368,32 @@ def test_more_tensors_than_a_launch_takes():
         blocks += (n + 255) // 256
 
 
+LISTS = {"short": SIZES, "one value": [(1,)], "full": [(64 * 256,)], "over": [(64 * 256,), (1,)], "many": [(3,)] * 241, "most": [(256,)] * 64, "sixteen": [(64 * 512,)],
+         "long": [(300000,), (7,), (0,), (65537,)]}
+
+
+@pytest.mark.parametrize("sizes", LISTS)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-def test_norm_and_clip(dtype):
+def test_norm_and_clip(dtype, sizes):
+    """Lists on both sides of what one workgroup takes by itself (64 blocks of 16 bytes a lane)."""
     from coarse3d_amd import ops
-    g = [rand(s, 3.0, 60 + i, dtype) for i, s in enumerate(SIZES)]
+    g = [rand(s, 3.0, 60 + i, dtype) for i, s in enumerate(LISTS[sizes])]
     total = math.sqrt(sum(float((x.double() ** 2).sum()) for x in g))
     norm, scale = ops.grad_norm(g)
     assert abs(float(norm) / total - 1) <= 2 * U and float(scale) == 1.0
     old = [x.clone() for x in g]
     versions = [x._version for x in g]
-    n2 = ops.clip_grad_norm_(g, 2.5)
+    limit = total * 0.4
+    n2 = ops.clip_grad_norm_(g, limit)
     assert float(n2) == float(norm) and all(x._version > v for x, v in zip(g, versions))
-    f = 2.5 / (total + 1e-6)
+    f = limit / (total + 1e-6)
     for a, b in zip(g, old):
         want = b.double() * f
         assert ((a.double() - want).abs() <= (HALF[dtype] * 1.01 + 3 * U) * want.abs() + (2.0 ** -25 if dtype == torch.float16 else 0)).all()
     old = [x.clone() for x in g]
     ops.clip_grad_norm_(g, 1e9)
     assert all(torch.equal(a, b) for a, b in zip(g, old))
-    assert float(ops.clip_grad_norm_(g, 0.0)) > 2 and all(not x.any() for x in g)
+    assert abs(float(ops.clip_grad_norm_(g, 0.0)) / limit - 1) < 0.01 and all(not x.any() for x in g)
 
 
 def test_norm_of_what_fp32_squares_lose():
@@ -431,6 +438,9 @@ def test_on_another_stream_and_two_graphs():
     g = [rand(s, 1.0, 5 + i) for i, s in enumerate(SIZES)]
     keep = [x.clone() for x in g]
     want = ops.grad_norm(g, 1.0)
+    off = torch.zeros(4000, device="cuda")[1:3501]           # an address off the vector grid
+    off.normal_()
+    assert abs(float(ops.grad_norm([off])[0]) / float(off.double().norm()) - 1) <= 2 * U
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):

@@ -1,7 +1,7 @@
 """ops.group_norm / group_norm_bwd against the formulas in float64.
 
-Tolerances.  u = 2^-24 is half a unit in the last place of fp32 relative to the value.  On the tested sizes no fp32 sum of the kernels adds
-more than 300 terms one after the other (longer ones are joined in 64 bits), so a mean of values bounded by A is off by at most 300 u A, and
+Tolerances.  u = 2^-24 is half a unit in the last place of fp32 relative to the value.  No fp32 sum of the kernels adds more than 300
+terms one after the other (256 of a thread and the joining of a workgroup's threads; longer ones are joined in 64 bits), so a mean of values bounded by A is off by at most 300 u A, and
 so are the others (variance: twice, it is a mean of squares of deviations that are themselves off; its root halves that again).  With
 A = max |x - mean| in units of sigma the normalised value is off by (300 + 300 A^2 + 8) u relative to its largest magnitude; the affine map and
 the activation (slope at most 1.1) add a few u of their own magnitudes.  A result in 16 bits adds half a unit of its type, eps / 2, of itself."""
@@ -281,9 +281,15 @@ def test_more_than_2_31_elements():
 
 
 def test_long_rows_keep_their_accuracy():
-    """A sample of half a million pixels: the sums are longer than the tolerance's 300 terms, so it is held to 1e-5 of the value directly."""
+    """Samples of half a million and of two million pixels: the mean error of long sums stays that of short ones (the worst case is 300 u =
+    2e-5 of the terms; in the 2-norm over many independent roundings a tenth of it is far from reached)."""
+    for shape in ((1, 64, 8192, 8), (1, 1, 2100003, 2)):
+        long_rows(shape)
+
+
+def long_rows(shape):
     from coarse3d_amd import ops
-    x, gamma, beta, dy = make((1, 64, 8192, 8), torch.float32, 2, seed=12, offset=2.0)
+    x, gamma, beta, dy = make(shape, torch.float32, 2, seed=12, offset=2.0)
     y, mean, rstd = ops.group_norm(x, 2, gamma, beta, act="lrelu")
     dx, dgamma, dbeta = ops.group_norm_bwd(dy, x, mean, rstd, gamma, beta, act="lrelu")
     o = oracle(x, dy, 2, gamma, beta, 1e-5, "lrelu", 0.01)
