@@ -3,7 +3,8 @@
 Layout: ``csrc/`` hand-written HIP kernels + the C ABI (``include/coarse3d_hip.h``),
 ``_lib`` the ctypes binding, ``ops`` tensor-level wrappers, ``backbone`` the fused
 SalsaNext forward/backward plan, ``pc_processor`` the mirror of the reference module API,
-``trainer`` the step orchestration, ``dist`` the data-parallel exchange points.
+``trainer`` the step orchestration, ``dist`` the data-parallel exchange points, ``optim`` the optimisers and
+gradient clipping, ``group_norm`` GroupNorm with an activation.
 """
 __version__ = "0.1.0"
 
