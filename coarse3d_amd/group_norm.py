@@ -50,5 +50,6 @@ class GroupNormAct(nn.Module):
     def forward(self, x):
         if x.dim() != 4 or x.shape[1] != self.num_channels:
             raise ValueError(f"GroupNormAct: expected [B, {self.num_channels}, H, W], got {tuple(x.shape)}")
-        y = group_norm_act(ops.to_nhwc(x), self.num_groups, self.weight, self.bias, self.eps, self.act, self.negative_slope)
+        w, b = (None, None) if self.weight is None else (self.weight.float(), self.bias.float())      # (a module moved to 16 bits)
+        y = group_norm_act(ops.to_nhwc(x), self.num_groups, w, b, self.eps, self.act, self.negative_slope)
         return ops.from_nhwc(y)

@@ -284,6 +284,20 @@ def test_group_norm_gradients_only_where_asked():
         assert not group_norm_act(x, 4, w).requires_grad
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_group_norm_module_in_16_bits(dtype):
+    from coarse3d_amd.group_norm import GroupNormAct
+    torch.manual_seed(4)
+    m = GroupNormAct(4, 24, act="silu").to(DEV, dtype)
+    x = torch.randn(2, 24, 6, 10, device=DEV, dtype=dtype, requires_grad=True)
+    y = m(x)
+    y.square().sum().backward()
+    ref = nn.functional.silu(nn.functional.group_norm(x.detach().double(), 4))
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    assert y.dtype == dtype and ((y.double() - ref).abs() <= 1.01 * half * ref.abs() + 2000 * U).all()
+    assert x.grad.dtype == dtype and m.weight.grad.dtype == dtype and torch.isfinite(m.weight.grad).all()
+
+
 def test_projector_with_group_norm_like_torch():
     from coarse3d_amd.pc_processor.models import ProjectionV1
     torch.manual_seed(6)
