@@ -6,12 +6,15 @@
 // group_norm, group_norm_bwd: checks, results and the call.  From Python one call cost 16 us of host time, and the kernel of a small
 // image takes 4.
 // Tensors that a call is about to write are marked as changed (autograd's version counters).  Nothing is kept from one call to the next.
+#define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <string>
 #include <vector>
 
@@ -75,8 +78,9 @@ std::string shape_of(at::IntArrayRef v) {
   for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
   return s + (v.size() == 1 ? ",)" : ")");
 }
+// (a view that stands for the negative of what its memory holds is not)
+bool own_memory(const at::Tensor& t) { return t.layout() == at::kStrided && !t.is_meta() && !t.is_quantized() && !t.is_neg(); }
 std::string type_of(const at::Tensor& t) { return std::string("torch.") + c10::toString(t.scalar_type()); }
-
 
 // ---------------------------------------------------------------- lists of tensors
 
@@ -168,7 +172,7 @@ struct Lists {
         };
         if (!THPVariable_Check(o)) throw Refused{what + names[s] + "[" + std::to_string(i) + "] is not a tensor", true};
         const at::Tensor& t = THPVariable_Unpack(o);
-        need(t.layout() == at::kStrided && !t.is_meta() && !t.is_quantized(), "is not a dense tensor with memory of its own");
+        need(own_memory(t), "is not a dense tensor with memory of its own");
         if (i == 0) type[s] = t.scalar_type();
         need(t.scalar_type() == type[s], "has another type than the first of its list");
         if (!seen) device = t.device();
@@ -244,7 +248,7 @@ PyObject* adamw(PyObject*, PyObject* args) {
     require(!l.have[6] || (l.type[6] == at::kFloat && l.type[0] != at::kFloat),
             what + "master copies are fp32, of 16-bit parameters; got " + l.type_name(6) + " of " + l.type_name(0));
     require(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0, what + "betas are in [0, 1), got (" + std::to_string(b1) + ", " + std::to_string(b2) + ")");
-    require(eps >= 0.0, what + "eps is not negative, got " + std::to_string(eps));
+    require(eps == 0.0 || (float)eps >= FLT_MIN, what + "eps is 0 or at least 2^-126, got " + c10::str(eps));
     c3d_adamw_desc d{};
     if (THPVariable_Check(lr_o)) {
       d.lr_dev = scalar(THPVariable_Unpack(lr_o), l.device, what + "lr");
@@ -277,6 +281,27 @@ PyObject* adamw(PyObject*, PyObject* args) {
     const int rc = lib.adamw_step(l.rec.data(), (int)l.rec.size(), &d, reinterpret_cast<c3d_stream>(stream));
     if (rc) return failed("c3d_adamw_step", rc);
     Py_RETURN_NONE;
+  });
+}
+
+// grads_of(params) -> (their gradients, None where there is none; a byte for each: its type, 255 without)
+PyObject* grads_of(PyObject*, PyObject* params) {
+  if (!PyList_Check(params) && !PyTuple_Check(params)) return fail(PyExc_TypeError, "grads_of: a list of tensors is expected");
+  return guarded([&]() -> PyObject* {
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(params);
+    std::string types((size_t)n, '\xff');
+    THPObjectPtr out(PyList_New(n));
+    if (!out) return nullptr;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* o = PySequence_Fast_GET_ITEM(params, i);
+      if (!THPVariable_Check(o)) throw Refused{"grads_of: a list of tensors is expected", true};
+      const at::Tensor& g = THPVariable_Unpack(o).grad();
+      if (g.defined()) types[(size_t)i] = (char)g.scalar_type();
+      PyObject* w = THPVariable_Wrap(g);       // (None for an undefined one)
+      if (!w) return nullptr;
+      PyList_SET_ITEM(out.get(), i, w);
+    }
+    return Py_BuildValue("Ny#", out.release(), types.data(), n);
   });
 }
 
@@ -315,7 +340,7 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
 const at::Tensor& tensor(PyObject* o, const char* what) {
   if (!THPVariable_Check(o)) throw Refused{std::string(what) + " is not a tensor", true};
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (t.layout() != at::kStrided || t.is_meta()) throw Refused{std::string(what) + " is not a dense tensor with memory of its own"};
+  if (!own_memory(t)) throw Refused{std::string(what) + " is not a dense tensor with memory of its own"};
   return t;
 }
 
@@ -461,6 +486,7 @@ PyObject* group_norm_bwd(PyObject*, PyObject* args) {
 PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, "bind({name: address}): the entry points of the loaded library"},
                          {"adamw", adamw, METH_VARARGS,
                           "adamw(what, lists, bits, step, lr, beta1, beta2, eps, weight_decay, grad_scale, seed, stream)"},
+                         {"grads_of", grads_of, METH_O, "grads_of(params) -> (gradients or None, a byte for each: its type)"},
                          {"grad_norm", grad_norm, METH_VARARGS, "grad_norm(what, grads, max_norm, clip, stream) -> (norm, scale)"},
                          {"group_norm", group_norm, METH_VARARGS, "group_norm(x, groups, gamma, beta, eps, act, slope, stream) -> (y, mean, rstd)"},
                          {"group_norm_bwd", group_norm_bwd, METH_VARARGS,

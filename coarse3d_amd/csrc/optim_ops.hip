@@ -1,9 +1,9 @@
 // Operators over the many tensors of an optimiser: the global norm of the gradients, their clipping, and the AdamW step with
-// states in 32 bits or in 8 bits.  All of them stream: nothing is read twice, and what bounds them is HBM.
+// states in 32 bits or in 8 bits.  All of them stream, and what bounds them is HBM.
 //
 // A call takes a host array of tensor records.  Records travel as kernel arguments (at most 4 KB a launch), so that nothing is
-// copied to the device ahead of the launch and a captured launch carries its own table; each workgroup finds its record by a
-// binary search over the records' first workgroups.
+// copied to the device ahead of the launch and a captured launch carries its own table; each wave finds the record of its blocks by
+// a vote of its lanes over the records' first blocks.
 //
 // AdamW (decoupled weight decay, step t, beta1 = b1, beta2 = b2):
 //     m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2,   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
@@ -851,7 +851,8 @@ extern "C" int c3d_adamw_step(const c3d_opt_tensor* t, int count, const c3d_adam
   C3D_REQUIRE(d->grad_type == 0 || d->grad_type == d->param_type, "adamw: gradients are fp32 or of the parameters' type");
   C3D_REQUIRE(!(d->has_master && d->param_type == 0), "adamw: fp32 parameters have no master copy");
   C3D_REQUIRE(d->beta1 >= 0.0 && d->beta1 < 1.0 && d->beta2 >= 0.0 && d->beta2 < 1.0, "adamw: betas are in [0, 1)");
-  C3D_REQUIRE(d->eps >= 0.0, "adamw: eps is negative");
+  // (the reciprocal instruction takes a smaller one for 0, and 0 / eps would not be 0)
+  C3D_REQUIRE(d->eps == 0.0 || (float)d->eps >= 0x1p-126f, "adamw: eps is 0 or at least 2^-126");
   C3D_REQUIRE(d->step_dev || d->step >= 1, "adamw: step counts from 1");
   if (int rc = check_records(t, count, 0xfu | (d->state_bits == 8 ? 0x30u : 0u) | (d->has_master ? 0x40u : 0u))) return rc;
   Hyper h;

@@ -25,9 +25,11 @@ embedding branch switches on.  A captured step (hipGraph) bakes the list of acti
 reference's optimiser (trainer.py:129, main.py:141,154): ``param_groups[0]["params"]`` indexes ALL parameters of the model
 in ``model.parameters()`` order (197 for SalsaNextProto: the frozen ``prototypes`` is index 0, ``feat_norm.*`` /
 ``mask_norm.*`` are 193-196), and ``state`` holds entries for the parameters that have been stepped."""
+import operator
+
 import torch
 
-from . import ops
+from . import _lib, ops
 from .ops import grad_norm
 
 
@@ -265,8 +267,9 @@ class AdamW(torch.optim.Optimizer):
         self.capturable, self.seed = capturable, seed
         self.last_grad_norm = None
         self.generation = 0
-        self._cohort_of = {}             # id(parameter) -> _Cohort
-        self._plan = None                # (which parameters have a gradient, [launch lists]) of the last step
+        self._native = _lib.native()
+        self._cohort_of = {}             # parameter -> _Cohort
+        self._plan = None                # (each group's parameters, their gradients' types, launch lists) of the last step
         self._lr_t = {}                  # group index -> (value seen, device scalar)
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
@@ -312,13 +315,13 @@ class AdamW(torch.optim.Optimizer):
                 if first is None:
                     first = _Cohort(0, torch.zeros((), device=p.device, dtype=torch.float32) if self.capturable else None)
                     self.generation += 1
-                self._cohort_of[id(p)] = first
+                self._cohort_of[p] = first
         # a cohort of which only some have a gradient: those get a counter of their own
-        idle = {id(self._cohort_of[id(p)]) for p, g in zip(params, grads) if g is None and id(p) in self._cohort_of}
+        idle = {id(self._cohort_of[p]) for p, g in zip(params, grads) if g is None and p in self._cohort_of}
         if not idle:
             return
         for p, g in zip(params, grads):
-            c = self._cohort_of.get(id(p))
+            c = self._cohort_of.get(p)
             if g is not None and id(c) in idle:
                 if id(c) not in halves:
                     if p.is_cuda and torch.cuda.is_current_stream_capturing():
@@ -326,7 +329,7 @@ class AdamW(torch.optim.Optimizer):
                                            "step in this configuration first")
                     halves[id(c)] = _Cohort(c.step, c.step_t.clone() if c.step_t is not None else None)
                     self.generation += 1
-                self._cohort_of[id(p)] = halves[id(c)]
+                self._cohort_of[p] = halves[id(c)]
 
     def _launches(self, grads_by_group):
         """[(group index, cohort, parameter indices, params, [state lists], masters)] of parameters with a gradient: one entry for each
@@ -336,12 +339,12 @@ class AdamW(torch.optim.Optimizer):
             for i, (p, g) in enumerate(zip(group["params"], grads)):
                 if g is not None:
                     master = "master" in self.state[p]
-                    runs.setdefault((gi, id(self._cohort_of[id(p)]), p.device, p.dtype, g.dtype, master), []).append(i)
+                    runs.setdefault((gi, id(self._cohort_of[p]), p.device, p.dtype, g.dtype, master), []).append(i)
         out = []
         for (gi, _, _, _, _, master), idx in runs.items():
             ps = [self.param_groups[gi]["params"][i] for i in idx]
             states = [None if name is None else [self.state[p][name] for p in ps] for name in self._STATE[self.state_bits]]
-            out.append((gi, self._cohort_of[id(ps[0])], idx, ps, states, [self.state[p]["master"] for p in ps] if master else None))
+            out.append((gi, self._cohort_of[ps[0]], idx, ps, states, [self.state[p]["master"] for p in ps] if master else None))
         return out
 
     @torch.no_grad()
@@ -350,12 +353,13 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        grads = [[p.grad for p in g["params"]] for g in self.param_groups]
-        active = [[None if x is None else x.dtype for x in g] for g in grads]
-        if self._plan is None or self._plan[0] != active:
-            self._split_cohorts([p for g in self.param_groups for p in g["params"]], [x for g in grads for x in g])
-            self._plan = (active, self._launches(grads))
-        launches = self._plan[1]
+        groups = [g["params"] for g in self.param_groups]
+        grads, types = zip(*map(self._native.grads_of, groups))
+        plan = self._plan
+        if plan is None or plan[1] != types or not all(all(map(operator.is_, a, b)) for a, b in zip(plan[0], groups)):
+            self._split_cohorts([p for g in groups for p in g], [x for g in grads for x in g])
+            plan = self._plan = ([list(g) for g in groups], types, self._launches(grads))
+        launches = plan[2]
         if not launches:
             return loss
         capturing = launches[0][3][0].is_cuda and torch.cuda.is_current_stream_capturing()
@@ -364,7 +368,7 @@ class AdamW(torch.optim.Optimizer):
                 raise RuntimeError("AdamW(capturable=True): the parameters are on several devices")
             if not capturing:
                 self.sync_lr()
-        lists = [[grads[gi][i] for i in idx] for gi, _, idx, _, _, _ in launches]
+        lists = [grads[gi] if len(idx) == len(grads[gi]) else [grads[gi][i] for i in idx] for gi, _, idx, _, _, _ in launches]
         scale = None
         if self.max_grad_norm is not None:
             scale = self._clip_factor(lists)
@@ -420,7 +424,7 @@ class AdamW(torch.optim.Optimizer):
 
     # ------------------------------------------------------------------ checkpoints
     def _step_of(self, p):
-        c = self._cohort_of.get(id(p))
+        c = self._cohort_of.get(p)
         return 0.0 if c is None else float(c.step_t) if c.step_t is not None else float(c.step)
 
     def state_dict(self):
@@ -441,6 +445,8 @@ class AdamW(torch.optim.Optimizer):
         if len(sd["param_groups"]) != len(self.param_groups) or any(
                 len(a["params"]) != len(b["params"]) for a, b in zip(sd["param_groups"], self.param_groups)):
             raise ValueError("AdamW.load_state_dict: the checkpoint's parameter groups differ from this optimiser's")
+        if any(g.get("amsgrad") or g.get("maximize") for g in sd["param_groups"]):
+            raise ValueError("AdamW.load_state_dict: the checkpoint is of an optimiser with amsgrad or maximize, which this one does not have")
         params = {}
         for a, b in zip(sd["param_groups"], self.param_groups):
             params.update(zip(a["params"], b["params"]))
@@ -479,7 +485,7 @@ class AdamW(torch.optim.Optimizer):
             self.state[p] = mine
             if (t, p.device) not in cohorts:
                 cohorts[t, p.device] = _Cohort(int(t), torch.full((), t, device=p.device, dtype=torch.float32) if self.capturable else None)
-            self._cohort_of[id(p)] = cohorts[t, p.device]
+            self._cohort_of[p] = cohorts[t, p.device]
         for g, s in zip(self.param_groups, sd["param_groups"]):
             g.update({k: tuple(v) if k == "betas" else v for k, v in s.items() if k in ("lr", "betas", "eps", "weight_decay", "initial_lr")})
         self._plan = None

@@ -122,3 +122,49 @@ def test_the_library_refuses_what_the_wrappers_would_not_send():
     for k in (dict(G=3), dict(N=-1), dict(HW=-1), dict(type=5), dict(act=9), dict(slope=2.0), dict(eps=-1.0), dict(x=None), dict(ws=None, HW=100000, ns=800000), dict(ps=7), dict(ns=23)):
         assert gn(**k) == 2, k
     assert gn(N=0) == 0 and gn(HW=0) == 0
+
+
+def test_negative_views_and_tiny_eps_are_refused():
+    """A tensor whose memory holds the negative of its values, and an eps that the reciprocal would take for 0."""
+    ops = _ops()
+    neg = torch._neg_view(torch.ones(4, 5))
+    with pytest.raises(ValueError, match=r"grads\[0\] is not a dense tensor"):
+        ops.grad_norm([neg])
+    with pytest.raises(ValueError, match="x is not a dense tensor"):
+        ops.group_norm(torch._neg_view(torch.ones(2, 3, 8)), 2)
+    for eps, match in ((1e-39, "2\\^-126"), (1e-60, "2\\^-126"), (float("nan"), "2\\^-126"), (-1e-8, "2\\^-126"), (0.0, "on cpu"), (2.0 ** -126, "on cpu")):
+        with pytest.raises(ValueError, match=match):
+            ops.adamw_step(_lists(), _lists(), _lists(), _lists(), step=1, lr=1e-3, eps=eps)
+
+
+def test_gradients_are_collected_with_their_types():
+    from coarse3d_amd import _lib as L
+    ps = [torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(2, dtype=torch.bfloat16)), torch.nn.Parameter(torch.ones(1))]
+    ps[0].grad, ps[1].grad = torch.ones(3), torch.ones(2, dtype=torch.bfloat16)
+    grads, types = L.native().grads_of(ps)
+    assert grads[0] is ps[0].grad and grads[1] is ps[1].grad and grads[2] is None
+    assert len(types) == 3 and types[2] == 255 and len(set(types)) == 3
+    assert L.native().grads_of([]) == ([], b"")
+    with pytest.raises(TypeError):
+        L.native().grads_of([1])
+
+
+def test_optimiser_replans_when_its_parameters_change():
+    """Parameters put in another's place are stepped (here: refused for being on the CPU) with states of their own; checkpoints with options
+    that this optimiser lacks are refused."""
+    from coarse3d_amd.optim import AdamW
+    ps = [torch.nn.Parameter(torch.ones(3)) for _ in range(2)]
+    opt = AdamW(ps, lr=0.1)
+    for p in ps:
+        p.grad = torch.ones(3)
+    with pytest.raises(ValueError, match="on cpu"):
+        opt.step()
+    new = torch.nn.Parameter(torch.ones(5))
+    new.grad = torch.ones(5)
+    opt.param_groups[0]["params"][1] = new
+    with pytest.raises(ValueError, match="on cpu"):
+        opt.step()
+    assert any(p is new for run in opt._plan[2] for p in run[3]) and opt.state[new]["exp_avg"].shape == (5,)
+    sd = torch.optim.AdamW(ps, amsgrad=True).state_dict()
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.load_state_dict(sd)

@@ -104,6 +104,18 @@ def test_against_float64(shape, groups, dtype, act):
     check(x, dy, groups, gamma, beta, act)
 
 
+# more channels than a workgroup takes: tiles of whole groups (the last one short), groups in several parts, both without a common vector,
+# a tile of one pixel
+WIDE = [((1, 30, 30, 2100), 100), ((2, 5, 9, 4104), 3), ((2, 3, 5, 8200), 2), ((1, 9, 70, 4099), 1), ((1, 70, 30, 4096), 32), ((1, 8, 9, 4095), 3)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", WIDE)
+def test_many_channels(shape, groups, dtype):
+    x, gamma, beta, dy = make(shape, dtype, groups, seed=shape[-1])
+    check(x, dy, groups, gamma, beta, "lrelu")
+
+
 @pytest.mark.parametrize("slope", [0.0, 0.1, 1.0])
 def test_slopes_and_no_affine(slope):
     x, _, _, dy = make((2, 9, 17, 24), torch.float32, 3, seed=5, affine=False)
