@@ -11,7 +11,7 @@
 //   large: a pass for the statistics, a pass that applies them.  The second walks the tensor backwards, so that it begins with what
 //          the first has left in the caches, and its workgroups fold the partial statistics of their sample by themselves.
 // One pass over x would need all workgroups of a sample to wait for one another; two passes cost a second read, most of it from the
-// infinity cache.  8x64x2048x32 fp32 forward: 26 us (5.1 TB/s) + 40 us (6.7 TB/s, read and written); 2x32x1024x704 bf16: forward 23 + 5 + 35,
+// infinity cache.  8x64x2048x32 fp32 forward: 26 us (5.1 TB/s) + 40 us (6.7 TB/s, read and written); 2x32x1024x704 bf16: forward 22 + 5 + 33,
 // backward 36 + 5 + 49.  A (sample, group) of 4096 bf16 values: 4 us, of 16384 fp32 ones 6 forward and 9 backward, latency all of it.
 #include <algorithm>
 #include <initializer_list>

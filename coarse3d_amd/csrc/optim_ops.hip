@@ -180,7 +180,7 @@ template <class T>
 constexpr int kRun = 64 * kLane<T>;                    // and a wave: their block
 
 // squares and sums in 64 bits (as many a clock as in 32 here): no gradient overflows, and the factor that other roundings depend on
-// is the same whatever the order of the sum.  One partial sum a workgroup.  38 MB: 12 us, 4 of them the launch's own.
+// is the same whatever the order of the sum.  One partial sum a workgroup.  38 MB: 13 us, 4 of them the launch's own.
 template <class T, class TB>
 __global__ __launch_bounds__(kNormThreads) void grad_sumsq_kernel(TB t, double* __restrict__ partial) {
   constexpr int V = kLane<T>, B = kRun<T>;
@@ -337,7 +337,7 @@ __device__ __forceinline__ void resolve(const Hyper& h, float& decay, float& ste
   }
 }
 
-// 28 bytes an fp32 element and some 20 operations: bound by HBM, 9.4 M parameters 53 us = 5.0 TB/s.
+// 28 bytes an fp32 element and some 20 operations: bound by HBM, 9.4 M parameters 52 us = 5.1 TB/s in two launches.
 template <class P, class G, bool MASTER, class TB>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(TB t, Hyper h) {
   using W = std::conditional_t<MASTER, float, P>;       // what carries the parameter's value
@@ -407,7 +407,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(TB t, Hyper h) {
 // it are exact.  Rounding is stochastic (16 bits an element, a hash of seed, step and the element's number): v moves by
 // 1 - b2 = 0.1 % a step, which is less than half a code step, and rounding to nearest would freeze it.
 //
-// 16 bytes an fp32 element, some 60 instructions: 41 M bf16 parameters with masters 139 us = 4.1 TB/s, 9.4 M fp32 ones 41 us = 3.7 TB/s
+// 16 bytes an fp32 element, some 60 instructions: 41 M bf16 parameters with masters 136 us = 4.8 TB/s, 9.4 M fp32 ones 41 us = 3.7 TB/s
 // in two launches of about 4 us of their own each.
 
 __device__ __forceinline__ uint32_t mix32(uint32_t h) {
