@@ -78,22 +78,30 @@ template <int V>
 constexpr int kSmallVecs = V == 8 ? 4 : 16 / V;        // vectors a thread holds
 // thread t: vector t % dv of the group's D / V, pixels t / dv + r * pl
 
-// sum over the workgroup, the same bits in every thread; red: 16 floats that the last sum did not use
-__device__ __forceinline__ float block_sum(float v, float* red) {
-#define C3D_SUM_STEP(ctrl, rows) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, rows, 0xf, false))
-  C3D_SUM_STEP(0x111, 0xf);      // row_shr:1, 2, 4, 8: lane 15 of a row of sixteen has the row's
-  C3D_SUM_STEP(0x112, 0xf);
-  C3D_SUM_STEP(0x114, 0xf);
-  C3D_SUM_STEP(0x118, 0xf);
-  C3D_SUM_STEP(0x142, 0xa);      // row_bcast:15 into rows 1 and 3, row_bcast:31 into 2 and 3: lane 63 has all
-  C3D_SUM_STEP(0x143, 0xc);
+// K sums over the workgroup, the same bits in every thread; red: K times 16 floats that the last sums did not use
+template <int K>
+__device__ __forceinline__ void block_sums(float (&v)[K], float* red) {
+#define C3D_SUM_STEP(ctrl, rows) v[k] += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v[k]), ctrl, rows, 0xf, false))
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    C3D_SUM_STEP(0x111, 0xf);    // row_shr:1, 2, 4, 8: lane 15 of a row of sixteen has the row's
+    C3D_SUM_STEP(0x112, 0xf);
+    C3D_SUM_STEP(0x114, 0xf);
+    C3D_SUM_STEP(0x118, 0xf);
+    C3D_SUM_STEP(0x142, 0xa);    // row_bcast:15 into rows 1 and 3, row_bcast:31 into 2 and 3: lane 63 has all
+    C3D_SUM_STEP(0x143, 0xc);
+  }
 #undef C3D_SUM_STEP
   const int nw = blockDim.x >> 6;
-  if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 63)
+#pragma unroll
+    for (int k = 0; k < K; ++k) red[(threadIdx.x >> 6) * K + k] = v[k];
   __syncthreads();
-  float s = 0.f;
-  for (int i = 0; i < nw; ++i) s += red[i];
-  return s;
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = 0.f;
+  for (int i = 0; i < nw; ++i)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += red[i * K + k];
 }
 
 template <class T, int V, int ACT>
@@ -102,7 +110,7 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_kernel(const T* __r
                                                                   float slope, T* __restrict__ y, float* __restrict__ mean,
                                                                   float* __restrict__ rstd) {
   constexpr int R = kSmallVecs<V>;
-  __shared__ float red[32];
+  __shared__ float red[48];
   const int n = blockIdx.x / G, g = blockIdx.x % G, l = threadIdx.x / dv, c = g * (C / G) + (threadIdx.x % dv) * V;
   const T* xs = x + n * xi.ns + c;
   Vec<T, V> raw[R];
@@ -116,25 +124,29 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_kernel(const T* __r
     be[e] = beta ? beta[c + e] : 0.f;
   }
   const float count = (float)HW * (float)(C / G);
-  float s = 0.f;
+  float first[1] = {0.f};
 #pragma unroll
   for (int r = 0; r < R; ++r)
     if (l < pl && l + r * pl < HW)
 #pragma unroll
-      for (int e = 0; e < V; ++e) s += (float)raw[r].v[e];
-  const float mu = block_sum(s, red) / count;
-  s = 0.f;
+      for (int e = 0; e < V; ++e) first[0] += (float)raw[r].v[e];
+  block_sums(first, red);
+  // about this mean, off by the rounding of its sum: what is left of the mean (a sum of small numbers) and the variance
+  const float mu = first[0] / count;
+  float s[2] = {0.f, 0.f};
 #pragma unroll
   for (int r = 0; r < R; ++r)
     if (l < pl && l + r * pl < HW)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float d = (float)raw[r].v[e] - mu;
-        s = fmaf(d, d, s);
+        s[0] += d;
+        s[1] = fmaf(d, d, s[1]);
       }
-  const float rs = 1.f / sqrtf(block_sum(s, red + 16) / count + eps);
+  block_sums(s, red + 16);
+  const float left = s[0] / count, var = s[1] / count - left * left, rs = 1.f / sqrtf((var < 0.f ? 0.f : var) + eps), off = -left * rs;
   if (threadIdx.x == 0) {
-    mean[blockIdx.x] = mu;
+    mean[blockIdx.x] = mu + left;
     rstd[blockIdx.x] = rs;
   }
   if (l >= pl) return;
@@ -144,7 +156,7 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_kernel(const T* __r
     if (l + r * pl < HW) {
       float o[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = act_fwd<ACT>(fmaf(((float)raw[r].v[e] - mu) * rs, ga[e], be[e]), slope);
+      for (int e = 0; e < V; ++e) o[e] = act_fwd<ACT>(fmaf(fmaf((float)raw[r].v[e] - mu, rs, off), ga[e], be[e]), slope);
       stv<T, V>(ys + (int64_t)(l + r * pl) * C, o);
     }
 }
@@ -159,7 +171,7 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_bwd_kernel(const T*
                                                                       float* __restrict__ dbeta) {
   constexpr int R = kSmallVecs<V>;
   extern __shared__ float2 rows[];                       // [pl][D], then [pl / 8][D]
-  __shared__ float red[32];
+  __shared__ float red[32];                              // 16 waves, two sums
   const int n = blockIdx.x / G, g = blockIdx.x % G, D = C / G, l = threadIdx.x / dv, q = threadIdx.x % dv, c = g * D + q * V;
   const T* xs = x + n * xi.ns + c;
   const T* ds = dy + n * di.ns + c;
@@ -188,14 +200,14 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_bwd_kernel(const T*
         a[e] += dz;
         b[e] = fmaf(dz, xh, b[e]);
       }
-  float s1 = 0.f, s2 = 0.f;
+  float s[2] = {0.f, 0.f};
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    s1 = fmaf(a[e], ga[e], s1);
-    s2 = fmaf(b[e], ga[e], s2);
+    s[0] = fmaf(a[e], ga[e], s[0]);
+    s[1] = fmaf(b[e], ga[e], s[1]);
   }
-  const float count = (float)HW * (float)D;
-  const float c1 = block_sum(s1, red) / count, c2 = block_sum(s2, red + 16) / count;
+  block_sums(s, red);
+  const float count = (float)HW * (float)D, c1 = s[0] / count, c2 = s[1] / count;
   if (l < pl) {
     T* os = dx + (int64_t)n * HW * C + c;
 #pragma unroll
