@@ -259,10 +259,9 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_bwd_kernel(const T*
 // ---------------------------------------------------------------- large: two passes
 
 // How an image is cut.  A tile of channels is `gpt` whole groups (split == 1), or one of `split` parts of a group too wide for a
-// workgroup; qt vectors wide, `pl` pixels side by side.  A sample's pixels are cut into runs of kRun * pl, and of nb workgroups the
+// workgroup; qt vectors wide, `pl` pixels side by side.  A sample's pixels are cut into runs of DEEP * pl, and of nb workgroups the
 // b-th takes runs b, b + nb, ...: at any time the workgroups read one window of memory together, and the second pass, which begins
 // with the last runs, finds the latest of it in the caches (8x64x2048x32 fp32, both passes: 82 us; with a chunk of its own each 86).
-constexpr int kRun = 4;
 struct Plan {
   int D, qt, pl, threads, tiles, gpt, split, nb;
   int64_t each;             // every workgroup takes this many runs, and the first `more` one more
@@ -320,23 +319,23 @@ __device__ __forceinline__ int64_t part_at(const Plan& p, int G, int n, int g) {
 
 // A thread's pixels of its workgroup's runs, all loads of a run in flight together; BACK: from the last run to the first.  (Fetching the
 // next run ahead as well costs the registers of a wave and loses 1-7 %.)
-template <bool BACK, class F>
+template <bool BACK, int DEEP, class F>
 struct Walk {
   using R = std::invoke_result_t<F, int64_t>;
   const Plan& p;
   int64_t HW;
   int b, l;
   F load;
-  R ahead[kRun];
+  R ahead[DEEP];
   // first pixel of the k-th run in the walk's order
   __device__ __forceinline__ int64_t at(int64_t k) const { return ((BACK ? runs_of(p, b) - 1 - k : k) * p.nb + b) * p.run + l; }
   __device__ __forceinline__ void fetch(int64_t i) {
-    if (i + (kRun - 1) * p.pl < HW) {
+    if (i + (DEEP - 1) * p.pl < HW) {
 #pragma unroll
-      for (int u = 0; u < kRun; ++u) ahead[u] = load(i + u * p.pl);
+      for (int u = 0; u < DEEP; ++u) ahead[u] = load(i + u * p.pl);
     } else {
 #pragma unroll
-      for (int u = 0; u < kRun; ++u)
+      for (int u = 0; u < DEEP; ++u)
         if (i + u * p.pl < HW) ahead[u] = load(i + u * p.pl);
     }
   }
@@ -348,20 +347,20 @@ struct Walk {
     for (int64_t k = 0; k < runs; ++k) {
       const int64_t i = at(k);
       if (k) fetch(i);
-      if (i + (kRun - 1) * p.pl < HW) {
+      if (i + (DEEP - 1) * p.pl < HW) {
 #pragma unroll
-        for (int u = 0; u < kRun; ++u) use(i + u * p.pl, ahead[u]);
+        for (int u = 0; u < DEEP; ++u) use(i + u * p.pl, ahead[u]);
       } else {
 #pragma unroll
-        for (int u = 0; u < kRun; ++u)
+        for (int u = 0; u < DEEP; ++u)
           if (i + u * p.pl < HW) use(i + u * p.pl, ahead[u]);
       }
     }
   }
 };
-template <bool BACK, class F>
-__device__ __forceinline__ Walk<BACK, F> walk(const Plan& p, int64_t HW, int b, int l, F load) {
-  return Walk<BACK, F>{p, HW, b, l, load};
+template <bool BACK, int DEEP, class F>
+__device__ __forceinline__ Walk<BACK, DEEP, F> walk(const Plan& p, int64_t HW, int b, int l, F load) {
+  return {p, HW, b, l, load};
 }
 
 // sums of s1, s2 [V] over the workgroup's `pl` pixel lanes: -> shared sum[ch] of the tile's channels
@@ -389,7 +388,7 @@ __device__ __forceinline__ void join_lanes(const Plan& p, const Tile& t, bool on
 
 // First pass: mean and sum of squared deviations of every group over the workgroup's pixels.  Values are shifted by its first pixel, so that a mean
 // far from zero costs nothing.
-template <class T, int V>
+template <class T, int V, int DEEP>
 __global__ __launch_bounds__(512) void gn_stats_kernel(const T* __restrict__ x, Img xi, Plan p, int64_t HW, int G, float2* __restrict__ part) {
   extern __shared__ float2 sum[];
   const Tile t = tile_of<V>(p, blockIdx.x % p.tiles, G);
@@ -401,7 +400,7 @@ __global__ __launch_bounds__(512) void gn_stats_kernel(const T* __restrict__ x, 
   for (int e = 0; e < V; ++e) shift[e] = s1[e] = s2[e] = 0.f;
   if (on) {
     const T* xs = x + n * xi.ns + t.c0 + q * V;
-    auto w = walk<false>(p, HW, b, l, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); });
+    auto w = walk<false, DEEP>(p, HW, b, l, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); });
     w.begin();
     ldv<T, V>(xs + (int64_t)b * p.run * xi.ps, shift);
     w.each([&](int64_t, const Vec<T, V>& r) {
@@ -468,7 +467,7 @@ __global__ __launch_bounds__(64) void gn_fold_kernel(const float2* __restrict__ 
 }
 
 // Second pass.  part != NULL: the statistics are still in pieces; every workgroup folds those of its groups
-template <class T, int V, int ACT, bool NT>
+template <class T, int V, int ACT, bool NT, int DEEP>
 __global__ __launch_bounds__(512) void gn_apply_kernel(const T* __restrict__ x, Img xi, Plan p, int64_t HW, int C, int G, const float2* __restrict__ part,
                                                       float eps, float* __restrict__ mean, float* __restrict__ rstd,
                                                       const float* __restrict__ gamma, const float* __restrict__ beta, float slope,
@@ -481,7 +480,7 @@ __global__ __launch_bounds__(512) void gn_apply_kernel(const T* __restrict__ x, 
   const bool on = l < p.pl && q < t.nq;
   const T* xs = x + n * xi.ns + t.c0 + q * V;
   T* ys = y + (int64_t)n * HW * C + t.c0 + q * V;
-  auto w = walk<true>(p, HW, b, l, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); });
+  auto w = walk<true, DEEP>(p, HW, b, l, [&](int64_t i) { return *reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps); });
   if (on) w.begin();
   for_groups(t.ng, [&](int g, int lane, int lanes) {
     const int k = n * G + t.g0 + min(g, t.ng - 1);
@@ -520,7 +519,7 @@ struct Two {
 };
 
 // Backward, first pass: per chunk and group (sum t, sum t xhat) -> part, and per channel (sum dz, sum dz xhat) -> chan [N][nb][C]
-template <class T, int V, int ACT>
+template <class T, int V, int ACT, int DEEP>
 __global__ __launch_bounds__(512) void gn_bwd_stats_kernel(const T* __restrict__ dy, Img di, const T* __restrict__ x, Img xi, Plan p, int64_t HW, int C,
                                                           int G, const float* __restrict__ mean, const float* __restrict__ rstd,
                                                           const float* __restrict__ gamma, const float* __restrict__ beta, float slope,
@@ -536,7 +535,7 @@ __global__ __launch_bounds__(512) void gn_bwd_stats_kernel(const T* __restrict__
   if (on) {
     const T* xs = x + n * xi.ns + t.c0 + q * V;
     const T* ds = dy + n * di.ns + t.c0 + q * V;
-    auto w = walk<false>(p, HW, b, l, [&](int64_t i) {
+    auto w = walk<false, DEEP>(p, HW, b, l, [&](int64_t i) {
       return Two<T, V>{*reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps), *reinterpret_cast<const Vec<T, V>*>(ds + i * di.ps)};
     });
     w.begin();
@@ -630,7 +629,7 @@ __global__ __launch_bounds__(256) void gn_channels_kernel(const float2* __restri
 }
 
 // Backward, second pass.  The first `extra` workgroups fold dgamma and dbeta; folded: part holds [N][G] means already
-template <class T, int V, int ACT, bool NT>
+template <class T, int V, int ACT, bool NT, int DEEP>
 __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(const T* __restrict__ dy, Img di, const T* __restrict__ x, Img xi, Plan p, int64_t HW, int N,
                                                           int C, int G, const float* __restrict__ mean, const float* __restrict__ rstd,
                                                           const float* __restrict__ gamma, const float* __restrict__ beta, float slope,
@@ -649,7 +648,7 @@ __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(const T* __restrict__
   const T* xs = x + n * xi.ns + t.c0 + q * V;
   const T* ds = dy + n * di.ns + t.c0 + q * V;
   T* os = dx + (int64_t)n * HW * C + t.c0 + q * V;
-  auto w = walk<true>(p, HW, b, l, [&](int64_t i) {
+  auto w = walk<true, DEEP>(p, HW, b, l, [&](int64_t i) {
     return Two<T, V>{*reinterpret_cast<const Vec<T, V>*>(xs + i * xi.ps), *reinterpret_cast<const Vec<T, V>*>(ds + i * di.ps)};
   });
   if (on) w.begin();
@@ -707,7 +706,26 @@ inline int vector_width(int esize, int C, int G, bool small, std::initializer_li
   return 1;
 }
 
-inline Plan make_plan(int N, int64_t HW, int C, int G, int V) {
+// Loads a thread has in flight together: `kDeep`, or more where they are narrow and memory would wait for requests.  Forward, odd channel
+// counts: 33 channels fp32 50 -> 40 us (bf16 46 -> 31), 301 37 -> 35 (33 -> 28); 2-byte loads 16 deep up to 128 vectors (33: 35 -> 31, 701:
+// 46 -> 50).  Backward with its two inputs: 33 channels 74 -> 60 (52 -> 47), 101 the same, 201 68 -> 72 (41 -> 46): up to 64 vectors only.
+// bytes: a load's; vectors: a pixel's
+struct DeepForward {
+  constexpr int operator()(int bytes, int vectors) const { return bytes >= 8 ? 4 : bytes == 2 && vectors <= 128 ? 16 : 8; }
+};
+struct DeepBackward {
+  constexpr int operator()(int bytes, int vectors) const { return bytes >= 8 || vectors > 64 ? 4 : 8; }
+};
+// f(depth, as a constant)
+template <int BYTES, class R, class F>
+int with_depth(R rule, int vectors, F f) {
+  constexpr int kNarrow = R()(BYTES, 1), kWide = R()(BYTES, 1 << 20);
+  if constexpr (kNarrow != kWide)
+    if (rule(BYTES, vectors) == kNarrow) return f(std::integral_constant<int, kNarrow>());
+  return f(std::integral_constant<int, kWide>());
+}
+
+inline Plan make_plan(int N, int64_t HW, int C, int G, int V, int deep) {
   Plan p;
   p.D = C / G;
   const int Q = C / V, u = V / gcd(p.D, V);
@@ -733,12 +751,12 @@ inline Plan make_plan(int N, int64_t HW, int C, int G, int V) {
   p.pl = most / p.qt > 1 ? most / p.qt : 1;
   p.threads = (p.qt * p.pl + 63) / 64 * 64;
   // about 1024 workgroups of 256 threads
-  p.run = kRun * p.pl;
+  p.run = deep * p.pl;
   const int64_t runs = (HW + p.run - 1) / p.run;
   int64_t want = 262144 / p.threads / ((int64_t)N * p.tiles);
   want = want < 1 ? 1 : want > 512 ? 512 : want;
-  // (at most 64 runs each, so that no fp32 sum of a thread has more than 256 terms)
-  const int64_t least = (runs + 63) / 64;
+  // (no fp32 sum of a thread has more than 256 terms)
+  const int64_t most_runs = 256 / deep, least = (runs + most_runs - 1) / most_runs;
   want = want < least ? least : want;
   p.nb = (int)(runs < want ? runs : want);
   p.each = runs / p.nb;
@@ -802,24 +820,27 @@ int forward(const T* x, Img xi, int N, int64_t HW, int C, int G, const float* ga
           C3D_CHECK_LAUNCH();
           return 0;
         }
-        const Plan p = make_plan(N, HW, C, G, V);
-        C3D_REQUIRE((int64_t)p.tiles * p.nb * N * p.threads < kMostThreads, "group_norm: too many samples and channels");
-        const dim3 grid((unsigned)(p.tiles * p.nb * N));
-        float2* part = reinterpret_cast<float2*>(ws);
-        const size_t lds = (size_t)(p.pl > 2 ? p.pl : 2) * p.qt * V * sizeof(float2);
-        hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(p.threads), lds, s, x, xi, p, HW, G, part);
-        C3D_CHECK_LAUNCH();
-        const bool fold = p.gpt * p.nb * p.split > kFoldMost;
-        if (fold) {
-          hipLaunchKernelGGL(gn_fold_kernel<V>, dim3(N * G), dim3(64), 0, s, part, p, HW, G, eps, mean, rstd);
+        return with_depth<V * sizeof(T)>(DeepForward(), C / V, [&](auto dd) {
+          constexpr int DEEP = decltype(dd)::value;
+          const Plan p = make_plan(N, HW, C, G, V, DEEP);
+          C3D_REQUIRE((int64_t)p.tiles * p.nb * N * p.threads < kMostThreads, "group_norm: too many samples and channels");
+          const dim3 grid((unsigned)(p.tiles * p.nb * N));
+          float2* part = reinterpret_cast<float2*>(ws);
+          const size_t lds = (size_t)(p.pl > 2 ? p.pl : 2) * p.qt * V * sizeof(float2);
+          hipLaunchKernelGGL((gn_stats_kernel<T, V, DEEP>), grid, dim3(p.threads), lds, s, x, xi, p, HW, G, part);
           C3D_CHECK_LAUNCH();
-        }
-        // (only whole vectors of 16 bytes have the form that goes past the caches)
-        const auto apply = V * sizeof(T) == 16 && past_caches(N, HW, C, sizeof(T)) ? gn_apply_kernel<T, V, A, V * sizeof(T) == 16> : gn_apply_kernel<T, V, A, false>;
-        hipLaunchKernelGGL(apply, grid, dim3(p.threads), p.gpt * sizeof(float2), s, x, xi, p, HW, C, G, fold ? nullptr : part, eps,
-                           mean, rstd, gamma, beta, slope, y);
-        C3D_CHECK_LAUNCH();
-        return 0;
+          const bool fold = p.gpt * p.nb * p.split > kFoldMost;
+          if (fold) {
+            hipLaunchKernelGGL(gn_fold_kernel<V>, dim3(N * G), dim3(64), 0, s, part, p, HW, G, eps, mean, rstd);
+            C3D_CHECK_LAUNCH();
+          }
+          // (only whole vectors of 16 bytes have the form that goes past the caches)
+          const auto apply = V * sizeof(T) == 16 && past_caches(N, HW, C, sizeof(T)) ? gn_apply_kernel<T, V, A, V * sizeof(T) == 16, DEEP> : gn_apply_kernel<T, V, A, false, DEEP>;
+          hipLaunchKernelGGL(apply, grid, dim3(p.threads), p.gpt * sizeof(float2), s, x, xi, p, HW, C, G, fold ? nullptr : part, eps,
+                             mean, rstd, gamma, beta, slope, y);
+          C3D_CHECK_LAUNCH();
+          return 0;
+        });
       });
     }
     return 2;
@@ -851,28 +872,31 @@ int backward(const T* dy, Img di, const T* x, Img xi, int N, int64_t HW, int C, 
           }
           return 0;
         }
-        const Plan p = make_plan(N, HW, C, G, V);
-        C3D_REQUIRE(((int64_t)p.tiles * p.nb * N + extra) * p.threads < kMostThreads, "group_norm_bwd: too many samples and channels");
-        const int blocks = p.tiles * p.nb * N;
-        float2* part = reinterpret_cast<float2*>(ws);
-        float2* chan = part + (int64_t)N * G * p.nb * p.split;
-        float2* coef = chan + (int64_t)N * p.nb * C;
-        const size_t lds = (size_t)(p.pl > 2 ? p.pl : 2) * p.qt * V * sizeof(float2);
-        hipLaunchKernelGGL((gn_bwd_stats_kernel<T, V, A>), dim3(blocks), dim3(p.threads), lds, s, dy, di, x, xi, p, HW, C, G, mean, rstd, gamma, beta,
-                           slope, part, wanted ? chan : nullptr);
-        C3D_CHECK_LAUNCH();
-        const bool fold = p.gpt * p.nb * p.split > kFoldMost;
-        if (fold) {
-          hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3(N * G), dim3(64), 0, s, part, p, HW, G, coef);
+        return with_depth<V * sizeof(T)>(DeepBackward(), C / V, [&](auto dd) {
+          constexpr int DEEP = decltype(dd)::value;
+          const Plan p = make_plan(N, HW, C, G, V, DEEP);
+          C3D_REQUIRE(((int64_t)p.tiles * p.nb * N + extra) * p.threads < kMostThreads, "group_norm_bwd: too many samples and channels");
+          const int blocks = p.tiles * p.nb * N;
+          float2* part = reinterpret_cast<float2*>(ws);
+          float2* chan = part + (int64_t)N * G * p.nb * p.split;
+          float2* coef = chan + (int64_t)N * p.nb * C;
+          const size_t lds = (size_t)(p.pl > 2 ? p.pl : 2) * p.qt * V * sizeof(float2);
+          hipLaunchKernelGGL((gn_bwd_stats_kernel<T, V, A, DEEP>), dim3(blocks), dim3(p.threads), lds, s, dy, di, x, xi, p, HW, C, G, mean, rstd, gamma, beta,
+                             slope, part, wanted ? chan : nullptr);
           C3D_CHECK_LAUNCH();
-        }
-        const size_t lds2 = std::max(p.gpt * sizeof(float2), wanted ? 8 * 16 * sizeof(double2) : 0);
-        const auto apply =
-            V * sizeof(T) == 16 && past_caches(N, HW, C, sizeof(T)) ? gn_bwd_apply_kernel<T, V, A, V * sizeof(T) == 16> : gn_bwd_apply_kernel<T, V, A, false>;
-        hipLaunchKernelGGL(apply, dim3(blocks + extra), dim3(p.threads), lds2, s, dy, di, x, xi, p, HW, N, C, G, mean, rstd, gamma,
-                           beta, slope, fold ? coef : part, (int)fold, chan, extra, dgamma, dbeta, dx);
-        C3D_CHECK_LAUNCH();
-        return 0;
+          const bool fold = p.gpt * p.nb * p.split > kFoldMost;
+          if (fold) {
+            hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3(N * G), dim3(64), 0, s, part, p, HW, G, coef);
+            C3D_CHECK_LAUNCH();
+          }
+          const size_t lds2 = std::max(p.gpt * sizeof(float2), wanted ? 8 * 16 * sizeof(double2) : 0);
+          const auto apply =
+              V * sizeof(T) == 16 && past_caches(N, HW, C, sizeof(T)) ? gn_bwd_apply_kernel<T, V, A, V * sizeof(T) == 16, DEEP> : gn_bwd_apply_kernel<T, V, A, false, DEEP>;
+          hipLaunchKernelGGL(apply, dim3(blocks + extra), dim3(p.threads), lds2, s, dy, di, x, xi, p, HW, N, C, G, mean, rstd, gamma,
+                             beta, slope, fold ? coef : part, (int)fold, chan, extra, dgamma, dbeta, dx);
+          C3D_CHECK_LAUNCH();
+          return 0;
+        });
       });
     }
     return 2;
@@ -899,9 +923,11 @@ extern "C" int64_t c3d_group_norm_ws_floats(int N, int64_t HW, int C, int G, int
     if (C % v) continue;
     const int D = C / G, u = v / gcd(D, v);
     if (!(C / v <= kMostVectors || (int64_t)u * D / v <= kMostVectors || D % v == 0)) continue;
-    const Plan p = make_plan(N, HW, C, G, v);
-    const int64_t f = 2 * ((int64_t)N * G * p.nb * p.split + (int64_t)N * p.nb * C + (int64_t)N * G);
-    most = f > most ? f : most;
+    for (int deep : {DeepForward()(v * (type == 0 ? 4 : 2), C / v), DeepBackward()(v * (type == 0 ? 4 : 2), C / v)}) {
+      const Plan p = make_plan(N, HW, C, G, v, deep);
+      const int64_t f = 2 * ((int64_t)N * G * p.nb * p.split + (int64_t)N * p.nb * C + (int64_t)N * G);
+      most = f > most ? f : most;
+    }
   }
   return most;
 }
