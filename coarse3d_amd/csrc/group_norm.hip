@@ -11,8 +11,8 @@
 //   large: a pass for the statistics, a pass that applies them.  The second walks the tensor backwards, so that it begins with what
 //          the first has left in the caches, and its workgroups fold the partial statistics of their sample by themselves.
 // One pass over x would need all workgroups of a sample to wait for one another; two passes cost a second read, most of it from the
-// infinity cache.  8x64x2048x32 fp32 forward: 26 us (5.1 TB/s) + 40 us (6.7 TB/s, read and written); 2x32x1024x704 bf16: forward 22 + 5 + 33,
-// backward 36 + 5 + 49.  A (sample, group) of 4096 bf16 values: 4 us, of 16384 fp32 ones 6 forward and 9 backward, latency all of it.
+// infinity cache.  8x64x2048x32 fp32 forward: 26 us (5.1 TB/s) + 40 us (6.7 TB/s, read and written); 2x32x1024x704 bf16: forward 21 + 5 + 34,
+// backward 36 + 5 + 46.  A (sample, group) of 4096 bf16 values: 4 us, of 16384 fp32 ones 6 forward and 9 backward, latency all of it.
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(kSmallThreads<V>) void gn_small_bwd_kernel(const T*
 // How an image is cut.  A tile of channels is `gpt` whole groups (split == 1), or one of `split` parts of a group too wide for a
 // workgroup; qt vectors wide, `pl` pixels side by side.  A sample's pixels are cut into runs of DEEP * pl, and of nb workgroups the
 // b-th takes runs b, b + nb, ...: at any time the workgroups read one window of memory together, and the second pass, which begins
-// with the last runs, finds the latest of it in the caches (8x64x2048x32 fp32, both passes: 82 us; with a chunk of its own each 86).
+// with the last runs, finds the latest of it in the caches (8x64x2048x32 fp32: with a chunk of its own each, both passes take 5 % longer).
 struct Plan {
   int D, qt, pl, threads, tiles, gpt, split, nb;
   int64_t each;             // every workgroup takes this many runs, and the first `more` one more
@@ -594,29 +594,33 @@ __global__ __launch_bounds__(64) void gn_bwd_fold_kernel(const float2* __restric
   if (threadIdx.x == 0) coef[blockIdx.x] = r;
 }
 
-// dgamma, dbeta of 16 channels: the rows of chan [rows][C], in 64 bits and a fixed order
+// dgamma, dbeta of 8 channels: the rows of chan [rows][C], in 64 bits and a fixed order.  Latency is all of it, and where the second pass
+// is short these workgroups are its end: many lanes a channel and many loads in flight (8x32x1024x64 fp32, both calls: 94 -> 92 us from 16
+// channels and 4 loads)
+constexpr int kFoldChannels = 8;
 __device__ __forceinline__ void fold_channels(const float2* __restrict__ chan, int64_t rows, int C, int c0, float* __restrict__ dgamma,
                                               float* __restrict__ dbeta, double2* red) {
-  const int c = c0 + (threadIdx.x & 15), lanes = blockDim.x / 16;
+  const int k = threadIdx.x % kFoldChannels, c = c0 + k, lanes = blockDim.x / kFoldChannels;
   double a = 0.0, b = 0.0;
   if (c < C)
-#pragma unroll 4
-    for (int64_t r = threadIdx.x / 16; r < rows; r += lanes) {
+#pragma unroll 8
+    for (int64_t r = threadIdx.x / kFoldChannels; r < rows; r += lanes) {
       const float2 v = chan[r * C + c];
       a += (double)v.x;
       b += (double)v.y;
     }
-  a += __shfl_xor(a, 16, 64);
-  b += __shfl_xor(b, 16, 64);
-  a += __shfl_xor(a, 32, 64);
-  b += __shfl_xor(b, 32, 64);
-  if ((threadIdx.x & 63) < 16) red[(threadIdx.x >> 6) * 16 + (threadIdx.x & 15)] = make_double2(a, b);
+#pragma unroll
+  for (int o = kFoldChannels; o < 64; o *= 2) {
+    a += __shfl_xor(a, o, 64);
+    b += __shfl_xor(b, o, 64);
+  }
+  if ((threadIdx.x & 63) < kFoldChannels) red[(threadIdx.x >> 6) * kFoldChannels + k] = make_double2(a, b);
   __syncthreads();
-  if (threadIdx.x < 16 && c < C) {
+  if (threadIdx.x < kFoldChannels && c < C) {
     a = b = 0.0;
     for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
-      a += red[w * 16 + threadIdx.x].x;
-      b += red[w * 16 + threadIdx.x].y;
+      a += red[w * kFoldChannels + k].x;
+      b += red[w * kFoldChannels + k].y;
     }
     if (dbeta) dbeta[c] = (float)a;
     if (dgamma) dgamma[c] = (float)b;
@@ -624,8 +628,8 @@ __device__ __forceinline__ void fold_channels(const float2* __restrict__ chan, i
 }
 __global__ __launch_bounds__(256) void gn_channels_kernel(const float2* __restrict__ chan, int64_t rows, int C, float* __restrict__ dgamma,
                                                          float* __restrict__ dbeta) {
-  __shared__ double2 red[8 * 16];
-  fold_channels(chan, rows, C, blockIdx.x * 16, dgamma, dbeta, red);
+  __shared__ double2 red[4 * kFoldChannels];
+  fold_channels(chan, rows, C, blockIdx.x * kFoldChannels, dgamma, dbeta, red);
 }
 
 // Backward, second pass.  The first `extra` workgroups fold dgamma and dbeta; folded: part holds [N][G] means already
@@ -637,7 +641,7 @@ __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(const T* __restrict__
                                                           float* __restrict__ dgamma, float* __restrict__ dbeta, T* __restrict__ dx) {
   extern __shared__ float2 stat[];
   if ((int)blockIdx.x < extra) {
-    fold_channels(chan, (int64_t)N * p.nb, C, blockIdx.x * 16, dgamma, dbeta, reinterpret_cast<double2*>(stat));
+    fold_channels(chan, (int64_t)N * p.nb, C, blockIdx.x * kFoldChannels, dgamma, dbeta, reinterpret_cast<double2*>(stat));
     return;
   }
   const int block = backwards(blockIdx.x - extra, gridDim.x - extra);
@@ -688,8 +692,8 @@ inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 constexpr int kMostVectors = 512;      // of a tile: its threads
 constexpr int64_t kMostThreads = (int64_t)1 << 32;   // of a launch
-// Partial results that a workgroup of the second pass folds by itself: 2048 of them beat a launch for it (8x32x1024x64 fp32, the pair:
-// 95 us to 98), 9344 do not (2x32x1024x704 bf16: 164 to 148)
+// Partial results that a workgroup of the second pass folds by itself: 3760 of them beat a launch for it (2x30000x128 bf16, 16 groups, forward:
+// 21.2 us to 21.9), 12000 do not (1x9000x704 bf16, 32 groups: 31.6 to 22.3)
 constexpr int kFoldMost = 4096;
 
 // widest vector that the channels, the strides and every pointer allow
@@ -706,7 +710,7 @@ inline int vector_width(int esize, int C, int G, bool small, std::initializer_li
   return 1;
 }
 
-// Loads a thread has in flight together: `kDeep`, or more where they are narrow and memory would wait for requests.  Forward, odd channel
+// Loads a thread has in flight together: 4, or more where they are narrow and memory would wait for requests.  Forward, odd channel
 // counts: 33 channels fp32 50 -> 40 us (bf16 46 -> 31), 301 37 -> 35 (33 -> 28); 2-byte loads 16 deep up to 128 vectors (33: 35 -> 31, 701:
 // 46 -> 50).  Backward with its two inputs: 33 channels 74 -> 60 (52 -> 47), 101 the same, 201 68 -> 72 (41 -> 46): up to 64 vectors only.
 // bytes: a load's; vectors: a pixel's
@@ -725,7 +729,7 @@ int with_depth(R rule, int vectors, F f) {
   return f(std::integral_constant<int, kWide>());
 }
 
-inline Plan make_plan(int N, int64_t HW, int C, int G, int V, int deep) {
+inline Plan make_plan(int N, int64_t HW, int C, int G, int V, int deep, bool narrow) {
   Plan p;
   p.D = C / G;
   const int Q = C / V, u = V / gcd(p.D, V);
@@ -750,15 +754,20 @@ inline Plan make_plan(int N, int64_t HW, int C, int G, int V, int deep) {
   const int most = p.qt > 128 ? 512 : 256;
   p.pl = most / p.qt > 1 ? most / p.qt : 1;
   p.threads = (p.qt * p.pl + 63) / 64 * 64;
-  // about 1024 workgroups of 256 threads
+  // Workgroups: two of 256 threads a CU saturate HBM with loads of 8 and 16 bytes, and what a workgroup costs beside them (its partial
+  // results, and folding everybody's) counts double with twice as many (13x1777x320 bf16, 32 groups: 26 us forward and 42 backward with four a
+  // CU, 21 and 27 with two); narrow loads want four (2x12000x701 bf16: 29 and 41 us, 37 and 57 with two).  All take equally many runs but for the
+  // last, if need be with an eighth more workgroups: the slowest decides (11x20000x40 bf16: 23 and 37 us as even as the numbers come, 20 and 26 so)
   p.run = deep * p.pl;
   const int64_t runs = (HW + p.run - 1) / p.run;
-  int64_t want = 262144 / p.threads / ((int64_t)N * p.tiles);
+  int64_t want = (narrow ? 262144 : 131072) / p.threads / ((int64_t)N * p.tiles);
   want = want < 1 ? 1 : want > 512 ? 512 : want;
   // (no fp32 sum of a thread has more than 256 terms)
   const int64_t most_runs = 256 / deep, least = (runs + most_runs - 1) / most_runs;
   want = want < least ? least : want;
-  p.nb = (int)(runs < want ? runs : want);
+  int64_t each = (runs - want / 8 + want - 1) / want;
+  each = each < 1 ? 1 : each;
+  p.nb = (int)((runs + each - 1) / each);
   p.each = runs / p.nb;
   p.more = (int)(runs % p.nb);
   p.last = (int)((runs - 1) % p.nb);
@@ -822,7 +831,7 @@ int forward(const T* x, Img xi, int N, int64_t HW, int C, int G, const float* ga
         }
         return with_depth<V * sizeof(T)>(DeepForward(), C / V, [&](auto dd) {
           constexpr int DEEP = decltype(dd)::value;
-          const Plan p = make_plan(N, HW, C, G, V, DEEP);
+          const Plan p = make_plan(N, HW, C, G, V, DEEP, V * sizeof(T) < 8);
           C3D_REQUIRE((int64_t)p.tiles * p.nb * N * p.threads < kMostThreads, "group_norm: too many samples and channels");
           const dim3 grid((unsigned)(p.tiles * p.nb * N));
           float2* part = reinterpret_cast<float2*>(ws);
@@ -855,7 +864,7 @@ int backward(const T* dy, Img di, const T* x, Img xi, int N, int64_t HW, int C, 
     constexpr int V = decltype(vv)::value;
     if constexpr (V * sizeof(T) <= 16) {
       const bool wanted = dgamma || dbeta;
-      const int extra = wanted ? ((C + 15) / 16 + 7) / 8 * 8 : 0;      // of eights, so that a chunk keeps its XCD
+      const int extra = wanted ? ((C + kFoldChannels - 1) / kFoldChannels + 7) / 8 * 8 : 0;      // of eights, so that a chunk keeps its XCD
       return with_act(act, [&](auto aa) {
         constexpr int A = decltype(aa)::value;
         if (small) {
@@ -867,14 +876,14 @@ int backward(const T* dy, Img di, const T* x, Img xi, int N, int64_t HW, int C, 
                              gamma, beta, slope, dx, (int)wanted, chan, dgamma, dbeta);
           C3D_CHECK_LAUNCH();
           if (wanted && N > 1) {
-            hipLaunchKernelGGL(gn_channels_kernel, dim3((C + 15) / 16), dim3(256), 0, s, chan, (int64_t)N, C, dgamma, dbeta);
+            hipLaunchKernelGGL(gn_channels_kernel, dim3((C + kFoldChannels - 1) / kFoldChannels), dim3(256), 0, s, chan, (int64_t)N, C, dgamma, dbeta);
             C3D_CHECK_LAUNCH();
           }
           return 0;
         }
         return with_depth<V * sizeof(T)>(DeepBackward(), C / V, [&](auto dd) {
           constexpr int DEEP = decltype(dd)::value;
-          const Plan p = make_plan(N, HW, C, G, V, DEEP);
+          const Plan p = make_plan(N, HW, C, G, V, DEEP, V * sizeof(T) < 8);
           C3D_REQUIRE(((int64_t)p.tiles * p.nb * N + extra) * p.threads < kMostThreads, "group_norm_bwd: too many samples and channels");
           const int blocks = p.tiles * p.nb * N;
           float2* part = reinterpret_cast<float2*>(ws);
@@ -889,7 +898,7 @@ int backward(const T* dy, Img di, const T* x, Img xi, int N, int64_t HW, int C, 
             hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3(N * G), dim3(64), 0, s, part, p, HW, G, coef);
             C3D_CHECK_LAUNCH();
           }
-          const size_t lds2 = std::max(p.gpt * sizeof(float2), wanted ? 8 * 16 * sizeof(double2) : 0);
+          const size_t lds2 = std::max(p.gpt * sizeof(float2), wanted ? 8 * kFoldChannels * sizeof(double2) : 0);
           const auto apply =
               V * sizeof(T) == 16 && past_caches(N, HW, C, sizeof(T)) ? gn_bwd_apply_kernel<T, V, A, V * sizeof(T) == 16, DEEP> : gn_bwd_apply_kernel<T, V, A, false, DEEP>;
           hipLaunchKernelGGL(apply, dim3(blocks + extra), dim3(p.threads), lds2, s, dy, di, x, xi, p, HW, N, C, G, mean, rstd, gamma,
@@ -924,7 +933,7 @@ extern "C" int64_t c3d_group_norm_ws_floats(int N, int64_t HW, int C, int G, int
     const int D = C / G, u = v / gcd(D, v);
     if (!(C / v <= kMostVectors || (int64_t)u * D / v <= kMostVectors || D % v == 0)) continue;
     for (int deep : {DeepForward()(v * (type == 0 ? 4 : 2), C / v), DeepBackward()(v * (type == 0 ? 4 : 2), C / v)}) {
-      const Plan p = make_plan(N, HW, C, G, v, deep);
+      const Plan p = make_plan(N, HW, C, G, v, deep, v * (type == 0 ? 4 : 2) < 8);
       const int64_t f = 2 * ((int64_t)N * G * p.nb * p.split + (int64_t)N * p.nb * C + (int64_t)N * G);
       most = f > most ? f : most;
     }
