@@ -273,6 +273,15 @@ class AdamW(torch.optim.Optimizer):
         self._lr_t = {}                  # group index -> (value seen, device scalar)
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    _OWN = ("state_bits", "master_weights", "max_grad_norm", "capturable", "seed", "last_grad_norm", "generation", "_cohort_of", "_lr_t")
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), **{k: self.__dict__[k] for k in self._OWN})
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plan, self._native = None, _lib.native()
+
     @property
     def graph_safe(self):
         """Whether ``TrainStep(graph=True)`` may capture the update."""

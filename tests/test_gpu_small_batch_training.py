@@ -144,6 +144,38 @@ def test_clipping_on_load_equals_clipping_ahead():
     assert float(optim.clip_grad_norm_([nn.Parameter(torch.ones(2, device=DEV))], 1.0)) == 0.0
 
 
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_copied_or_saved_optimiser_goes_on_alike(capturable):
+    import copy
+    import io
+    from coarse3d_amd.optim import AdamW
+    torch.manual_seed(6)
+    net = nn.Sequential(nn.Linear(40, 33), nn.Linear(33, 7)).to(DEV)
+    opt = AdamW(net.parameters(), lr=1e-2, state_bits=8, max_grad_norm=0.7, capturable=capturable, seed=5)
+    x = torch.randn(9, 40, device=DEV)
+
+    def step(n, o, which=slice(None)):
+        for p in n.parameters():
+            p.grad = None
+        n(x).square().sum().backward()
+        for p in list(n.parameters())[which]:
+            p.grad = None
+        o.step()
+    step(net, opt, slice(0, 1))                    # (two cohorts)
+    step(net, opt, slice(0, 0))
+    file = io.BytesIO()
+    torch.save((net, opt), file)                   # (pickle by itself cannot take torch's 8-bit floats)
+    file.seek(0)
+    others = [copy.deepcopy((net, opt)), torch.load(file, weights_only=False)]
+    for _ in range(3):
+        step(net, opt, slice(0, 0))
+    for n, o in others:
+        for _ in range(3):
+            step(n, o, slice(0, 0))
+        assert all(torch.equal(a, b) for a, b in zip(net.parameters(), n.parameters()))
+        assert [float(v["step"]) for v in o.state_dict()["state"].values()] == [float(v["step"]) for v in opt.state_dict()["state"].values()]
+
+
 def test_optimiser_refusals():
     from coarse3d_amd.optim import AdamW
     p = [nn.Parameter(torch.ones(3, device=DEV))]
